@@ -217,6 +217,122 @@ typedef struct fa2_rope_params {
 
 int fa2_rope_f16(const fa2_rope_params *p, int32_t backward, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators on token rows: what a decoder runs between two attention calls and
+ * after the last one.  Tensors are rows of elements with unit stride; a row
+ * stride is in elements.
+ * ------------------------------------------------------------------------- */
+enum fa2_dtype { FA2_F16 = 0, FA2_BF16 = 1, FA2_F32 = 2, FA2_E4M3 = 3 /* OCP 8-bit: 4 exponent, 3 mantissa bits */ };
+
+/* Largest row fa2_rms_norm_* and the largest hidden size fa2_xent_* take. */
+#define FA2_ROW_MAX 16384
+
+/* RMS norm with the residual's addition (reference @ None: train.py:1862-1875 and
+ * the additions of train.py:1986-1994, there separate torch calls):
+ *   h = residual + D(x), rounded to the residual's type  (h = x without residual)
+ *   y = h * (mean(h^2) + eps)^-1/2 * weight
+ * D is dropout with probability dropout_p (fa2_dropout's, same seed and counter;
+ * needs a residual), statistics are fp32.  y_type FA2_E4M3 leaves y in 8 bits: per
+ * row scale = max(amax|y| / 448, 2^-126) in `scale` and e4m3(y / scale) in y; a row
+ * whose y holds NaN has scale NaN.
+ * Types: x fp16, bf16 or fp32; residual and h of x's type or fp32; y of x's type or
+ * e4m3, and any where x is fp32; weight any but e4m3.  h, y, rstd (fp32 [rows],
+ * kept for the backward; may be NULL) and scale are packed: row stride = cols.
+ * 1 <= cols <= FA2_ROW_MAX, rows < 2^31. */
+typedef struct fa2_rms_norm_params {
+    const void *x, *residual, *weight;   /* residual NULL: none                */
+    void *h, *y;                         /* h: required with a residual        */
+    float *rstd, *scale;                 /* scale: FA2_E4M3 only               */
+    int64_t x_stride, residual_stride;
+    int64_t rows;
+    int32_t cols;
+    int32_t x_type, residual_type, weight_type, y_type;
+    float eps;
+    float dropout_p;
+    uint32_t seed;
+} fa2_rms_norm_params;
+
+int fa2_rms_norm_fwd(const fa2_rms_norm_params *p, void *stream);
+
+/* Gradients of fa2_rms_norm_fwd (not of its 8-bit form).  dh NULL: none comes in
+ * through h.  dx, dresidual, dweight are packed; each may be NULL where it is not
+ * wanted.  h and h_type are those of the forward (x's without a residual).
+ * dweight is summed in a fixed order (results repeat bit for bit) through a
+ * workspace of fa2_rms_norm_bwd_workspace_bytes(rows, cols) bytes. */
+typedef struct fa2_rms_norm_bwd_params {
+    const void *dy, *dh, *h, *weight;
+    const float *rstd;
+    void *dx, *dresidual, *dweight;
+    int64_t dy_stride, dh_stride, h_stride;
+    int64_t rows;
+    int32_t cols;
+    int32_t x_type, h_type, weight_type, y_type;
+    float dropout_p;
+    uint32_t seed;
+} fa2_rms_norm_bwd_params;
+
+size_t fa2_rms_norm_bwd_workspace_bytes(int64_t rows, int32_t cols);
+int fa2_rms_norm_bwd(const fa2_rms_norm_bwd_params *p, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Dropout: y[r, c] = x[r, c] / (1 - p) where the generator keeps (r, c), else 0.
+ * The generator is the attention dropout's hash at row r, column c and head 0:
+ * counter-based, so the gradient is the same call on dy with the same seed, and no
+ * mask is stored.  y is packed; x and y of one type (fp16, bf16, fp32); rows and
+ * cols < 2^31. */
+typedef struct fa2_dropout_params {
+    const void *x;
+    void *y;
+    int64_t x_stride;
+    int64_t rows;
+    int32_t cols;
+    int32_t type;
+    float dropout_p;
+    uint32_t seed;
+} fa2_dropout_params;
+
+int fa2_dropout(const fa2_dropout_params *p, void *stream);
+
+/* Language model head with softmax cross entropy (reference @ None:
+ * train.py:2059-2082, there chunks of a linear layer and F.cross_entropy):
+ *   z = x weight^T,  loss_i = log sum_v exp z_iv - z_(i, target_i)
+ * over the tokens whose target is not ignore_index, without the [rows, vocab]
+ * logits being kept: the forward keeps one log-sum-exp a token and a packed copy of
+ * the states that count (`state`), the backward forms the logits again piece by
+ * piece of the vocabulary.  Tokens that do not count take no part in any product:
+ * their loss and their dx are 0 whatever their states hold.  A target outside the
+ * vocabulary gives NaN.  reduction: one loss a token (0 where ignored), their sum,
+ * or the mean over the tokens that count (NaN where there is none).
+ * x, weight, dx, dweight: fp16 or bf16; dx and dweight packed; logits, log-sum-exp
+ * and all sums fp32.  weight 16-byte aligned with weight_stride a multiple of 8,
+ * unless hidden is no multiple of 64 (then it is copied to padded rows first).
+ * rows <= 2^24, vocab <= 2^24, 1 <= hidden <= FA2_ROW_MAX.  Nothing is atomic:
+ * results repeat bit for bit. */
+enum fa2_reduction { FA2_REDUCE_NONE = 0, FA2_REDUCE_SUM = 1, FA2_REDUCE_MEAN = 2 };
+
+typedef struct fa2_xent_params {
+    const void *x, *weight;
+    const int64_t *target;               /* [rows]                             */
+    int64_t x_stride, weight_stride;
+    int64_t rows;
+    int32_t hidden, vocab;
+    int32_t type;
+    int32_t reduction;
+    int64_t ignore_index;
+    float *loss;                         /* forward: [rows] (none), else [1]   */
+    void *state;                         /* written by the forward, read by the
+                                            backward: fa2_xent_state_bytes     */
+    size_t state_bytes;
+    const float *dloss;                  /* backward: gradient of loss         */
+    int64_t dloss_stride;                /* none: elements between its rows    */
+    void *dx, *dweight;                  /* backward: each NULL if not wanted  */
+} fa2_xent_params;
+
+size_t fa2_xent_state_bytes(int64_t rows, int32_t hidden);
+size_t fa2_xent_fwd_workspace_bytes(int64_t rows, int32_t hidden, int32_t vocab);
+size_t fa2_xent_bwd_workspace_bytes(int64_t rows, int32_t hidden, int32_t vocab);
+int fa2_xent_fwd(const fa2_xent_params *p, void *workspace, size_t workspace_bytes, void *stream);
+int fa2_xent_bwd(const fa2_xent_params *p, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Human-readable text for a status code, and the detail message of the last
  * failing call on this host thread ("" if none). */
 const char *fa2_status_string(int status);

@@ -27,7 +27,8 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
-HIP_SOURCES = ["fa2_fwd.hip", "fa2_bwd.hip", "fa2_rope.hip", "fa2_capi.hip"]
+HIP_SOURCES = ["fa2_fwd.hip", "fa2_bwd.hip", "fa2_rope.hip", "fa2_norm.hip", "fa2_dropout.hip", "fa2_xent.hip",
+               "fa2_capi.hip", "fa2_token_capi.hip"]
 LIB_NAME = "libfa2_mi355x.so"
 EXT_NAME = "_fa2_torch"
 
@@ -92,7 +93,7 @@ def build_extension(verbose=False):
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=" + EXT_NAME,
         "-DTORCH_API_INCLUDE_EXTENSION_H", "-D_GLIBCXX_USE_CXX11_ABI=" + str(int(torch._C._GLIBCXX_USE_CXX11_ABI)),
         *[f"-I{p}" for p in inc],
-        os.path.join(CSRC, "torch_binding.cpp"),
+        os.path.join(CSRC, "torch_binding.cpp"), os.path.join(CSRC, "torch_binding_tokens.cpp"),
         "-o", tmp,
         f"-L{torch_lib}", f"-L{LIB}",
         "-lfa2_mi355x", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",

@@ -19,6 +19,9 @@ namespace {
 
 thread_local char g_err[512] = {0};
 
+}  // namespace
+
+namespace fa2 {
 int fail(int status, const char *fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
@@ -26,6 +29,12 @@ int fail(int status, const char *fmt, ...) {
     va_end(ap);
     return status;
 }
+void clear_error() { g_err[0] = 0; }
+}  // namespace fa2
+
+namespace {
+
+using fa2::fail;
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

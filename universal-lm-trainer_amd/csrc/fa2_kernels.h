@@ -184,6 +184,11 @@ inline bool decode_streams(const FwdArgs &a, bool causal) {
 // keys 8.0 against 7.2).
 inline int decode_waves(const FwdArgs &a) { return a.split_keys <= 256 ? 4 : 8; }
 
+// Sets the calling thread's error message (fa2_last_error) and returns `status`;
+// clear_error empties it, first thing in every entry point.
+int fail(int status, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+void clear_error();
+
 // Compute units of the current device (cached per device; 256 on MI355X).
 // Launchers use it to size grids against the slots of two workgroups per CU.
 int device_cus();

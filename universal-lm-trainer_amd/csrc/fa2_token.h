@@ -1,0 +1,203 @@
+// fa2_token.h -- argument blocks, launch entry points and device helpers of the
+// operators that work on token rows [rows, cols]: RMS norm with the residual's
+// addition (fa2_norm.hip), dropout (fa2_dropout.hip) and the language model
+// head with its cross entropy (fa2_xent.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/fa2_mi355x.h"
+#include "fa2_device.h"
+
+namespace fa2 {
+
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+struct vec_of;
+template <>
+struct vec_of<_Float16> {
+    typedef h4 v4;
+    typedef h8 v8;
+};
+template <>
+struct vec_of<__bf16> {
+    typedef b4 v4;
+    typedef b8 v8;
+};
+template <>
+struct vec_of<float> {
+    typedef f4 v4;
+    typedef f8 v8;
+};
+
+struct NormFwdArgs {
+    const void *x, *res, *w;     // res null: h = x
+    void *h, *y;                 // h null: not stored
+    float *rstd, *scale;         // rstd null: not stored; scale: 8-bit output only
+    int64_t x_stride, res_stride;
+    int64_t rows;
+    int cols;
+    float eps;
+    int w_type;
+    int vec;                     // every row of every tensor takes four-element loads
+    uint32_t seed_part;          // dropout_row_part(seed, -1, 0): the hash's terms of seed and head
+    uint32_t drop_thr;           // 0: no dropout
+    float inv_keep;
+};
+
+struct NormBwdArgs {
+    const void *dy, *dh, *h, *w; // dh null: no gradient through h
+    const float *rstd;
+    void *dx, *dres;             // dres null: not wanted
+    void *dw;                    // null: not wanted
+    float *part;                 // [blocks, cols] partial sums of dw
+    int64_t dy_stride, dh_stride, h_stride;
+    int64_t rows;
+    int cols;
+    int w_type, dw_type;
+    int vec;
+    int blocks;
+    uint32_t seed_part, drop_thr;
+    float inv_keep;
+};
+
+struct DropoutArgs {
+    const void *x;
+    void *y;
+    int64_t x_stride, rows;
+    int cols;
+    int vec;
+    uint32_t seed_part, drop_thr;
+    float inv_keep;
+};
+
+// Language model head with cross entropy.  Token rows that count (target not
+// ignore_index) are packed to the front: packed row j is token rowmap[j], rows
+// are `rows_pad` (a multiple of XENT_PAD) with zeros behind the last one.
+constexpr int XENT_PAD = 256;      // packed rows and a piece's columns: multiples of this
+constexpr int XENT_KPAD = 64;      // the hidden size the products see: a multiple of this
+
+struct XentArgs {
+    int64_t rows;                  // N
+    int rows_pad;
+    int d, dp;                     // hidden size; padded to XENT_KPAD
+    int V;
+    int type;
+    const void *x;                 // [N, d]
+    int64_t x_stride;
+    const void *w;                 // [V, dp]: the weight, or its padded copy
+    int64_t w_stride;
+    const int64_t *target;
+    int64_t ignore;
+    int reduction;
+    // kept for the backward
+    int *count;                    // [0]: rows that count
+    int *pos;                      // [N]: packed row of a token, -1 where ignored
+    int *rowmap;                   // [rows_pad]
+    int *tgt;                      // [rows_pad]: target, -1 where it is outside the vocabulary
+    float *lse;                    // [rows_pad]
+    void *xc;                      // [rows_pad, dp]
+    // forward
+    int splits;                    // slices of the vocabulary
+    float *part;                   // [splits, rows_pad, 2]: maximum and sum of a row in a slice
+    float *row_loss;               // [rows_pad]
+    float *loss;                   // scalar, or [N]
+    // backward
+    const float *g;                // gradient of loss
+    int g_stride;                  // none: elements between rows of g (0: one for all)
+    float *coef;                   // [rows_pad]: factor of a row of P
+    float *unscale;                // [1]: factor of the finished products
+    int piece;                     // vocabulary columns of a piece
+    int v0, v1;                    // the piece
+    void *P;                       // [rows_pad, piece]
+    int ksplit;                    // dX: slices of a piece, each with sums of its own
+    float *acc;                    // [ksplit, rows_pad, d]
+    bool first;                    // dX: the first piece starts the sums
+    void *dx, *dw;                 // [N, d], [V, d]; null: not wanted
+};
+
+hipError_t launch_xent_pack(const XentArgs &a, hipStream_t st);
+hipError_t launch_xent_fwd(const XentArgs &a, hipStream_t st);
+hipError_t launch_xent_pad_weight(const void *w, int64_t w_stride, void *out, int V, int d, int dp, int type, hipStream_t st);
+hipError_t launch_xent_bwd_prepare(const XentArgs &a, hipStream_t st);
+hipError_t launch_xent_bwd_piece(const XentArgs &a, hipStream_t st);
+hipError_t launch_xent_bwd_finish(const XentArgs &a, hipStream_t st);
+
+hipError_t launch_norm_fwd(const NormFwdArgs &a, int x_type, int res_type, int y_type, hipStream_t st);
+hipError_t launch_norm_bwd(const NormBwdArgs &a, int x_type, int h_type, int y_type, hipStream_t st);
+int norm_bwd_blocks(int64_t rows, int cols);
+hipError_t launch_dropout(const DropoutArgs &a, int type, hipStream_t st);
+
+// v under dropout, for element (row, col): the attention's generator with head 0;
+// `part_row` holds the hash's terms of the seed, the head and the row.  A dropped
+// element is 0 whatever it was (inf and NaN too).
+__device__ __forceinline__ float drop(float v, uint32_t part_row, int col, uint32_t thr, float inv_keep) {
+    return dropout_keep_hashed(part_row ^ dropout_col_term(col), thr) ? v * inv_keep : 0.f;
+}
+
+// Four elements of a row from column col on, as fp32; zero past the row's end.
+template <typename T>
+__device__ __forceinline__ f4 load4(const T *row, int col, int cols, bool vec) {
+    f4 r = {0.f, 0.f, 0.f, 0.f};
+    if (vec) {
+        if (col < cols)
+            r = __builtin_convertvector(*reinterpret_cast<const typename vec_of<T>::v4 *>(row + col), f4);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col + j < cols) r[j] = (float)row[col + j];
+    }
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T *row, int col, int cols, bool vec, f4 v) {
+    const typename vec_of<T>::v4 q = __builtin_convertvector(v, typename vec_of<T>::v4);
+    if (vec) {
+        if (col < cols) *reinterpret_cast<typename vec_of<T>::v4 *>(row + col) = q;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col + j < cols) row[col + j] = q[j];
+    }
+}
+
+// The same with the element type as an argument (uniform).
+__device__ __forceinline__ f4 load4_typed(const void *row, int type, int col, int cols, bool vec) {
+    if (type == FA2_F16) return load4(static_cast<const _Float16 *>(row), col, cols, vec);
+    if (type == FA2_BF16) return load4(static_cast<const __bf16 *>(row), col, cols, vec);
+    return load4(static_cast<const float *>(row), col, cols, vec);
+}
+
+__device__ __forceinline__ void store1_typed(void *p, int type, int64_t i, float v) {
+    if (type == FA2_F16)
+        static_cast<_Float16 *>(p)[i] = (_Float16)v;
+    else if (type == FA2_BF16)
+        static_cast<__bf16 *>(p)[i] = (__bf16)v;
+    else
+        static_cast<float *>(p)[i] = v;
+}
+
+// Sum (or, MAX, the largest value, NaN first) over the G lanes that share a row;
+// G = 64: one wave, otherwise a whole workgroup, through `red` (one float a wave).
+template <int G, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float *red) {
+    auto join = [](float a, float b) FA2_INLINE { return MAX ? ((b > a || b != b) ? b : a) : a + b; };
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = join(v, __shfl_xor(v, o));
+    if (G > 64) {
+        __syncthreads();   // the previous use of red has been read
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < G / 64; ++i) v = join(v, red[i]);
+    }
+    return v;
+}
+
+}  // namespace fa2

@@ -30,6 +30,8 @@
 
 #include "../../include/fa2_mi355x.h"
 
+void bind_token_ops(pybind11::module_ &m);   // torch_binding_tokens.cpp
+
 namespace {
 
 void *current_stream(const torch::Tensor &t) {
@@ -378,5 +380,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           pybind11::arg("seed"), pybind11::arg("mode") = 7, pybind11::arg("mask") = pybind11::none());
     m.def("rope_fwd", &rope_fwd, "fused RoPE forward");
     m.def("rope_bwd", &rope_bwd, "fused RoPE backward");
+    bind_token_ops(m);
     m.def("version", []() { return std::string(fa2_version()); });
 }

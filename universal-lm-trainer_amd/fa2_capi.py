@@ -54,7 +54,52 @@ class RopeParams(ctypes.Structure):
     ]
 
 
-STRUCTS = {"fa2_fwd_params": FwdParams, "fa2_bwd_params": BwdParams, "fa2_rope_params": RopeParams}
+class RmsNormParams(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+        ("h", ctypes.c_void_p), ("y", ctypes.c_void_p), ("rstd", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64), ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int32), ("x_type", ctypes.c_int32), ("residual_type", ctypes.c_int32),
+        ("weight_type", ctypes.c_int32), ("y_type", ctypes.c_int32),
+        ("eps", ctypes.c_float), ("dropout_p", ctypes.c_float), ("seed", ctypes.c_uint32),
+    ]
+
+
+class RmsNormBwdParams(ctypes.Structure):
+    _fields_ = [
+        ("dy", ctypes.c_void_p), ("dh", ctypes.c_void_p), ("h", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+        ("rstd", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("dresidual", ctypes.c_void_p),
+        ("dweight", ctypes.c_void_p),
+        ("dy_stride", ctypes.c_int64), ("dh_stride", ctypes.c_int64), ("h_stride", ctypes.c_int64),
+        ("rows", ctypes.c_int64), ("cols", ctypes.c_int32), ("x_type", ctypes.c_int32), ("h_type", ctypes.c_int32),
+        ("weight_type", ctypes.c_int32), ("y_type", ctypes.c_int32), ("dropout_p", ctypes.c_float),
+        ("seed", ctypes.c_uint32),
+    ]
+
+
+class DropoutParams(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int32), ("type", ctypes.c_int32), ("dropout_p", ctypes.c_float), ("seed", ctypes.c_uint32),
+    ]
+
+
+class XentParams(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("target", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64), ("weight_stride", ctypes.c_int64), ("rows", ctypes.c_int64),
+        ("hidden", ctypes.c_int32), ("vocab", ctypes.c_int32), ("type", ctypes.c_int32), ("reduction", ctypes.c_int32),
+        ("ignore_index", ctypes.c_int64), ("loss", ctypes.c_void_p),
+        ("state", ctypes.c_void_p), ("state_bytes", ctypes.c_size_t),
+        ("dloss", ctypes.c_void_p), ("dloss_stride", ctypes.c_int64),
+        ("dx", ctypes.c_void_p), ("dweight", ctypes.c_void_p),
+    ]
+
+
+STRUCTS = {"fa2_fwd_params": FwdParams, "fa2_bwd_params": BwdParams, "fa2_rope_params": RopeParams,
+           "fa2_rms_norm_params": RmsNormParams, "fa2_rms_norm_bwd_params": RmsNormBwdParams,
+           "fa2_dropout_params": DropoutParams, "fa2_xent_params": XentParams}
+F16, BF16, F32, E4M3 = range(4)   # fa2_dtype
 
 
 def header_functions():
@@ -98,6 +143,23 @@ def load():
         lib.fa2_bwd_noalloc_scratch_bytes.restype = ctypes.c_size_t
         lib.fa2_rope_f16.argtypes = [ctypes.POINTER(RopeParams), ctypes.c_int32, ctypes.c_void_p]
         lib.fa2_rope_f16.restype = ctypes.c_int
+        lib.fa2_rms_norm_fwd.argtypes = [ctypes.POINTER(RmsNormParams), ctypes.c_void_p]
+        lib.fa2_rms_norm_fwd.restype = ctypes.c_int
+        lib.fa2_rms_norm_bwd_workspace_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32]
+        lib.fa2_rms_norm_bwd_workspace_bytes.restype = ctypes.c_size_t
+        lib.fa2_rms_norm_bwd.argtypes = [ctypes.POINTER(RmsNormBwdParams), ctypes.c_void_p, ctypes.c_size_t,
+                                         ctypes.c_void_p]
+        lib.fa2_rms_norm_bwd.restype = ctypes.c_int
+        lib.fa2_dropout.argtypes = [ctypes.POINTER(DropoutParams), ctypes.c_void_p]
+        lib.fa2_dropout.restype = ctypes.c_int
+        lib.fa2_xent_state_bytes.argtypes = [ctypes.c_int64, ctypes.c_int32]
+        lib.fa2_xent_state_bytes.restype = ctypes.c_size_t
+        for name in ("fa2_xent_fwd_workspace_bytes", "fa2_xent_bwd_workspace_bytes"):
+            getattr(lib, name).argtypes = [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]
+            getattr(lib, name).restype = ctypes.c_size_t
+        for name in ("fa2_xent_fwd", "fa2_xent_bwd"):
+            getattr(lib, name).argtypes = [ctypes.POINTER(XentParams), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
         lib.fa2_status_string.argtypes = [ctypes.c_int]
         lib.fa2_status_string.restype = ctypes.c_char_p
         lib.fa2_last_error.argtypes = []
