@@ -1,0 +1,228 @@
+// fa2_product.h -- matrix product tiles, D[m, n] = sum_k A[m, k] B[n, k], on the
+// 32x32x16 MFMAs: operands by direct global->LDS transfers, two stages of 64 k.
+//
+// Operands are 16-bit matrices in either order: ROWS are stored [m][k] (n for B),
+// the others [k][m].  A tile's operand is a number of panels of 64 x 64 elements (8
+// KB, rows of 128 bytes): 64 of its rows by 64 k, or 64 k rows by 64 columns.  Both
+// kinds are moved by the same transfers; they differ in the swizzle (16-byte chunk
+// ch of row r sits at ch ^ swz(r)) and in the read: ROWS fragments are 16-byte
+// reads, the others the transposing 8-byte reads, in the same k order (lane 32 g2 +
+// c holds k = 8 g2 .. 8 g2 + 7 of each step of 16), so that any two orders can meet
+// in one product.
+#pragma once
+
+#include "fa2_token.h"
+
+namespace fa2 {
+
+__device__ __forceinline__ f16x mfma(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f16x mfma(b8 a, b8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// Row of element r of a 32x32 accumulator (its column is lane & 31).
+__device__ __forceinline__ int acc_row(int r, int g2) { return 8 * (r >> 2) + 4 * g2 + (r & 3); }
+
+constexpr int PANEL = 8192;    // bytes
+constexpr int PK = 64;         // k of a stage
+
+// One operand of a tile: where the transfers of this thread read.  Eight waves
+// move a panel, wave w its rows 8 w .. 8 w + 7.
+template <bool ROWS, int NP>
+struct Feed {
+    uint64_t base;                 // ROWS: first row, k = 0; else k = 0, column 0
+    uint32_t ld;                   // bytes of a row
+    uint32_t off[ROWS ? NP : 1];   // this lane's bytes from base (ROWS: in each panel)
+    uint32_t col[ROWS ? 1 : NP];   // else: bytes of each panel's first column
+    int kleft;                     // else: k rows there are
+
+    // p: the matrix; first: the tile's first row (column); limit: rows (columns, a
+    // multiple of 64) there are, at least 1 (64); k rows klimit.  What lies past a limit is
+    // read from the last row or panel there is.
+    __device__ __forceinline__ void init(const void *p, int64_t ld_elems, int first, int limit, int klimit) {
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = 8 * w + (lane >> 3);
+        ld = (uint32_t)ld_elems * 2;
+        if constexpr (ROWS) {
+            const int f0 = min(first, limit - 1);
+            base = uniform((uint64_t)(uintptr_t)p + (uint64_t)f0 * (uint64_t)ld);
+            const uint32_t ch = (uint32_t)((lane & 7) ^ swz_rows(r)) << 4;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) off[j] = (uint32_t)min(64 * j + r, limit - 1 - f0) * ld + ch;
+        } else {
+            base = uniform((uint64_t)(uintptr_t)p);
+            off[0] = (uint32_t)((lane & 7) ^ swz_tr(r)) << 4;
+            kleft = klimit;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) col[j] = (uint32_t)min(first + 64 * j, limit - 64) * 2;
+        }
+    }
+
+    static __device__ __forceinline__ uint64_t uniform(uint64_t v) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+        return ((uint64_t)hi << 32) | lo;
+    }
+
+    // Starts the transfers of stage k0 / PK into the panels at LDS address `lds`.
+    __device__ __forceinline__ void issue(int k0, uint32_t lds) const {
+        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        lds += w * 1024;
+        if constexpr (ROWS) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) lds_dma16_at(base + (uint64_t)(uint32_t)k0 * 2, off[j], lds + j * PANEL);
+        } else {
+            const int r = 8 * (threadIdx.x >> 6) + ((threadIdx.x & 63) >> 3);
+            const uint32_t o = (uint32_t)min(r, kleft - 1 - k0) * ld + off[0];
+            const uint64_t b = base + (uint64_t)(uint32_t)k0 * ld;
+#pragma unroll
+            for (int j = 0; j < NP; ++j) lds_dma16_at(b + col[j], o, lds + j * PANEL);
+        }
+    }
+};
+
+// Fragment reads of one operand: 32 rows (columns) from `at` (a multiple of 32) of
+// the tile, k step ks of the stage.
+template <typename T, bool ROWS>
+struct Frag {
+    typedef typename vec_of<T>::v8 v8;
+    uint32_t off[4];   // ROWS: of k step 0..3; else: column 0 / 32 of a panel, first / second read
+
+    __device__ __forceinline__ void init() {
+        const int lane = threadIdx.x & 63;
+        if constexpr (ROWS) {
+            const int c = lane & 31, g2 = lane >> 5;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) off[ks] = (uint32_t)(c * 128 + (((2 * ks + g2) ^ swz_rows(c)) << 4));
+        } else {
+            const int G = lane >> 4, s = lane & 15;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = 8 * (G >> 1) + (s >> 2) + 4 * (q & 1), col = 32 * (q >> 1) + 16 * (G & 1) + 4 * (s & 3);
+                off[q] = (uint32_t)(row * 128 + (((col >> 3) ^ swz_tr(row)) << 4) + 2 * (col & 7));
+            }
+        }
+    }
+
+    __device__ __forceinline__ v8 read(const char *stage, int at, int ks) const {
+        typedef __attribute__((address_space(3))) const char lds_char;
+        lds_char *p = (lds_char *)stage + (at >> 6) * PANEL;
+        if constexpr (ROWS) {
+            return *(__attribute__((address_space(3))) const v8 *)(p + (at & 32) * 128 + off[ks]);
+        } else {
+            const int q = (at & 32) >> 4;
+            const s4v r0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v *)(p + ks * 2048 + off[q]));
+            const s4v r1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v *)(p + ks * 2048 + off[q + 1]));
+            return __builtin_bit_cast(v8, __builtin_shufflevector(r0, r1, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+};
+
+// Tile of 64 MP x 64 NP by eight waves in WM x WN, each (64 MP / WM) x (64 NP / WN).
+template <typename T, bool AROWS, bool BROWS, int MP, int NP, int WM, int WN>
+struct Product {
+    static_assert(WM * WN == 8, "eight waves");
+    static constexpr int TM = 64 * MP, TN = 64 * NP;
+    static constexpr int MI = TM / WM / 32, NI = TN / WN / 32;   // a wave's 32x32 blocks
+    static constexpr int STAGE = (MP + NP) * PANEL;
+    static constexpr int LDS = 2 * STAGE;
+
+    Feed<AROWS, MP> A;
+    Feed<BROWS, NP> B;
+    Frag<T, AROWS> fa;
+    Frag<T, BROWS> fb;
+    char *mem;
+    uint32_t lds;
+    int wm, wn;        // the wave's first row and column of the tile
+
+    __device__ __forceinline__ void init(char *m) {
+        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        mem = m;
+        lds = lds_addr(m);
+        wm = (w % WM) * (TM / WM);
+        wn = (w / WM) * (TN / WN);
+        fa.init();
+        fb.init();
+    }
+
+    __device__ __forceinline__ void issue(int k0, int stage) const {
+        A.issue(k0, lds + stage * STAGE);
+        B.issue(k0, lds + stage * STAGE + MP * PANEL);
+    }
+
+    __device__ __forceinline__ void compute(int stage, f16x (&acc)[MI][NI]) const {
+        typedef typename vec_of<T>::v8 v8;
+        const char *s = mem + stage * STAGE;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            v8 a[MI], b[NI];
+#pragma unroll
+            for (int i = 0; i < MI; ++i) a[i] = fa.read(s, wm + 32 * i, ks);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) b[j] = fb.read(s + MP * PANEL, wn + 32 * j, ks);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j]);
+        }
+    }
+
+    static __device__ __forceinline__ void zero(f16x (&acc)[MI][NI]) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = zero16();
+    }
+
+    // k from kbeg to kend, multiples of PK.  Leaves no transfer in flight and every
+    // wave past its last read.
+    __device__ __forceinline__ void run(int kbeg, int kend, f16x (&acc)[MI][NI]) const {
+        zero(acc);
+        if (kbeg < kend) issue(kbeg, 0);
+        int stage = 0;
+        for (int k = kbeg; k < kend; k += PK) {
+            vm_wait<0>();
+            lds_barrier();   // this stage has landed; every wave is done with the other
+            if (k + PK < kend) issue(k + PK, stage ^ 1);
+            compute(stage, acc);
+            stage ^= 1;
+        }
+        lds_barrier();
+    }
+};
+
+// store_rows_f16 for either 16-bit type: a wave's 32 x 64 block in two
+// accumulators (acc0: columns 0..31, acc1: 32..63, row = lane & 31), times mul, as
+// rows dst + r * stride for r < nrows, through 4 KB of LDS that only this wave
+// touches.  Columns from ncols on are left out (a multiple of 8 for whole 16-byte stores).
+template <typename T>
+__device__ __forceinline__ void store_rows(const f16x &acc0, const f16x &acc1, float mul, char *blk, T *dst, int64_t stride,
+                                           int nrows, int ncols, bool vec16) {
+    typedef typename vec_of<T>::v4 v4;
+    typedef typename vec_of<T>::v8 v8;
+    const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
+#pragma unroll
+    for (int db = 0; db < 2; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f4 x;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = (db ? acc1 : acc0)[4 * i + j] * mul;
+            *reinterpret_cast<v4 *>(blk + c * 128 + (((4 * db + i) ^ (c & 7)) << 4) + 8 * g2) = __builtin_convertvector(x, v4);
+        }
+    const int ch = lane & 7;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int r = 8 * k + (lane >> 3);
+        const v8 v = *reinterpret_cast<const v8 *>(blk + r * 128 + ((ch ^ (r & 7)) << 4));
+        if (r < nrows) {
+            T *p = dst + r * stride + 8 * ch;
+            if (vec16 && 8 * ch + 8 <= ncols) {
+                *reinterpret_cast<v8 *>(p) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (8 * ch + e < ncols) p[e] = v[e];
+            }
+        }
+    }
+}
+
+}  // namespace fa2

@@ -103,6 +103,7 @@ struct XentArgs {
     void *xc;                      // [rows_pad, dp]
     // forward
     int splits;                    // slices of the vocabulary
+    bool narrow;                   // tiles of 64 tokens, not 256
     float *part;                   // [splits, rows_pad, 2]: maximum and sum of a row in a slice
     float *row_loss;               // [rows_pad]
     float *loss;                   // scalar, or [N]

@@ -67,6 +67,7 @@ int check_norm_types(int x, int res, int y, bool fp8) {
 // ---------------------------------------------------------------------------
 struct XentPlan {
     int rows_pad, dp;
+    bool narrow;
     int splits, piece, ksplit;
     // offsets in the state
     size_t count, lse, tgt, rowmap, pos, xc, state_bytes;
@@ -81,14 +82,15 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     XentPlan p;
     p.rows_pad = (int)((rows + XENT_PAD - 1) / XENT_PAD * XENT_PAD);
     p.dp = (d + XENT_KPAD - 1) / XENT_KPAD * XENT_KPAD;
-    const int64_t R = p.rows_pad, nr = R / 128, nd = (d + 127) / 128, tiles = (V + 127) / 128;
+    const int64_t R = p.rows_pad, nd = (d + 255) / 256, tiles = (V + 255) / 256;
     auto clamp = [](int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; };
-    p.splits = (int)clamp(1024 / nr, 1, tiles);
+    p.narrow = R <= 1024;
+    p.splits = (int)clamp(256 / (p.narrow ? (rows + 63) / 64 : R / 256), 1, tiles);
     // A piece's P is at most 128 MiB, half of the Infinity Cache, in equal pieces.
     const int64_t most = clamp(((int64_t)128 << 20) / (2 * R) / XENT_PAD * XENT_PAD, XENT_PAD, 1 << 24);
     const int64_t pieces = (V + most - 1) / most;
     p.piece = (int)(((V + pieces - 1) / pieces + XENT_PAD - 1) / XENT_PAD * XENT_PAD);
-    p.ksplit = (int)clamp(512 / (nd * nr), 1, clamp(p.piece / 128, 1, 32));
+    p.ksplit = (int)clamp(256 / (nd * (R / 256)), 1, clamp(p.piece / 128, 1, 32));
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += up256(bytes); return o; };
     p.count = take(256);
@@ -127,6 +129,7 @@ int xent_check(const fa2_xent_params *p, const void *ws, size_t ws_bytes, bool b
     if ((rc = check_type("x", p->type, FA2_BF16))) return rc;
     if (p->reduction < 0 || p->reduction > FA2_REDUCE_MEAN) return fail(FA2_ERR_BAD_ARGUMENT, "reduction %d is not known", p->reduction);
     if ((rc = check_row_tensor("weight", p->weight, p->type, p->weight_stride))) return rc;
+    if (p->weight_stride >= 1 << 22) return fail(FA2_ERR_BAD_SHAPE, "weight row stride %lld is not below 2^22", (long long)p->weight_stride);
     if (p->weight_stride < p->hidden) return fail(FA2_ERR_BAD_SHAPE, "weight row stride %lld is below hidden", (long long)p->weight_stride);
     if (p->hidden % fa2::XENT_KPAD == 0 && (!aligned(p->weight, 16) || p->weight_stride % 8))
         return fail(FA2_ERR_MISALIGNED, "weight needs a 16-byte aligned base and a row stride that is a multiple of 8");
@@ -169,6 +172,7 @@ fa2::XentArgs xent_args(const fa2_xent_params *p, const XentPlan &pl) {
     a.pos = reinterpret_cast<int *>(s + pl.pos);
     a.xc = s + pl.xc;
     a.splits = pl.splits;
+    a.narrow = pl.narrow;
     a.piece = pl.piece;
     a.ksplit = pl.ksplit;
     return a;

@@ -20,17 +20,12 @@
 // the matrix units; the gradients themselves are rounded to the same type.  P is
 // scaled so that its largest possible value is 2^15: in fp16 probabilities down
 // to 2^-29 stay normal numbers.
-#include "fa2_token.h"
+#include "fa2_product.h"
 
 namespace fa2 {
 namespace {
 
 constexpr float P_SCALE = 32768.f;
-
-typedef unsigned int u4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ f16x mfma(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f16x mfma(b8 a, b8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
 // ---------------------------------------------------------------------------
 // Packing
@@ -106,82 +101,6 @@ __global__ __launch_bounds__(256) void xent_pad_weight_kernel(const T *w, int64_
 }
 
 // ---------------------------------------------------------------------------
-// A 128 x 128 tile of a product, D[m, n] = sum_k A[m, k] B[n, k], by four waves
-// of 64 x 64.  ROWS operands are stored [m][k], the others [k][m].  K is a
-// multiple of 32; rows (k rows of the others) at or past the given limit are
-// read from the last one, columns past the limit of the others likewise.
-// ---------------------------------------------------------------------------
-constexpr int TM = 128, TN = 128, TK = 32, TLD = TK + 8;
-
-template <typename T>
-struct Operand {
-    const T *p;
-    int64_t ld;
-    int first, limit;      // ROWS: first row of the tile, rows; else first column, columns (a multiple of 8)
-    int klimit;            // not ROWS: k rows
-};
-
-template <typename T, bool ROWS>
-__device__ __forceinline__ void stage(const Operand<T> &o, int k0, T (*s)[TLD]) {
-    typedef typename vec_of<T>::v8 v8;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int id = threadIdx.x + 256 * i;
-        if (ROWS) {
-            const int r = id >> 2, c = (id & 3) * 8;
-            const int64_t row = min(o.first + r, o.limit - 1);
-            *reinterpret_cast<v8 *>(&s[r][c]) = *reinterpret_cast<const v8 *>(o.p + row * o.ld + k0 + c);
-        } else {
-            const int k = id >> 4, c = (id & 15) * 8;
-            const int64_t row = min(k0 + k, o.klimit - 1);
-            const v8 v = *reinterpret_cast<const v8 *>(o.p + row * o.ld + min(o.first + c, o.limit - 8));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[c + e][k] = v[e];
-        }
-    }
-}
-
-template <typename T>
-struct TileMem {
-    T a[TM][TLD], b[TN][TLD];
-};
-
-template <typename T, bool AROWS, bool BROWS>
-__device__ __forceinline__ void product_tile(const Operand<T> &A, const Operand<T> &B, int kbeg, int kend, TileMem<T> &s,
-                                             f16x acc[2][2]) {
-    typedef typename vec_of<T>::v8 v8;
-    const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
-    const int wm = (threadIdx.x >> 6 & 1) * 64, wn = (threadIdx.x >> 7) * 64;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = zero16();
-    for (int k0 = kbeg; k0 < kend; k0 += TK) {
-        __syncthreads();
-        stage<T, AROWS>(A, k0, s.a);
-        stage<T, BROWS>(B, k0, s.b);
-        __syncthreads();
-#pragma unroll
-        for (int ks = 0; ks < TK; ks += 16) {
-            v8 fa[2], fb[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fa[i] = *reinterpret_cast<const v8 *>(&s.a[wm + 32 * i + c][ks + 8 * g2]);
-                fb[i] = *reinterpret_cast<const v8 *>(&s.b[wn + 32 * i + c][ks + 8 * g2]);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j]);
-        }
-    }
-}
-
-// Element (i, j, r) of a wave's accumulators: row m0 + 8 (r / 4) + 4 g2 + r % 4 of
-// the tile's M side, column c of its N side.
-__device__ __forceinline__ int acc_row(int r, int g2) { return 8 * (r >> 2) + 4 * g2 + (r & 3); }
-
-// ---------------------------------------------------------------------------
 // Forward
 // ---------------------------------------------------------------------------
 
@@ -194,56 +113,86 @@ __device__ __forceinline__ void join_max_sum(float &m, float &l, float m2, float
 
 // Maximum and sum of exp of each packed row over a slice of the vocabulary.  The
 // M side are vocabulary rows, the N side tokens: a lane holds one token's logits.
-template <typename T>
-__global__ __launch_bounds__(256) void xent_stats_kernel(const XentArgs a) {
-    __shared__ TileMem<T> s;
-    __shared__ float sm[2][TN], sl[2][TN];
-    const int nr = a.rows_pad / TN;
+// Each lane keeps a reference r and the sum of exp(z - r) of the logits it has
+// seen.  r is the maximum of the lane's first tile and moves only when a sum
+// passes 2^100: fp32 holds the terms of any larger logits until then.
+template <typename T, int NP, int WM, int WN>
+__global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
+    typedef Product<T, true, true, 4, NP, WM, WN> Pr;
+    constexpr int MI = Pr::MI, NI = Pr::NI;
+    __shared__ __align__(16) char mem[Pr::LDS];
+    const int nr = a.rows_pad / Pr::TN;
     const int rb = blockIdx.x % nr, split = blockIdx.x / nr;
-    if (rb * TN >= a.count[0]) return;
-    const int tiles = (a.V + TM - 1) / TM;
+    if (rb * Pr::TN >= a.count[0]) return;
+    const int tiles = (a.V + Pr::TM - 1) / Pr::TM;
     const int t0 = (int)((int64_t)tiles * split / a.splits), t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
-    const int wmi = threadIdx.x >> 6 & 1, wn = (threadIdx.x >> 7) * 64;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const Operand<T> B = {static_cast<const T *>(a.xc), a.dp, rb * TN, a.rows_pad, 0};
+    Pr pr;
+    pr.init(mem);
+    pr.B.init(a.xc, a.dp, rb * Pr::TN, a.rows_pad, 0);
+    float ref[NI], sum[NI];
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+        ref[j] = -INFINITY;
+        sum[j] = 0.f;
+    }
     for (int t = t0; t < t1; ++t) {
-        const Operand<T> A = {static_cast<const T *>(a.w), a.w_stride, t * TM, a.V, 0};
-        f16x acc[2][2];
-        product_tile<T, true, true>(A, B, 0, a.dp, s, acc);
+        f16x acc[MI][NI];
+        pr.A.init(a.w, a.w_stride, t * Pr::TM, a.V, 0);
+        pr.run(0, a.dp, acc);
+        if ((t + 1) * Pr::TM > a.V) {   // rows past the vocabulary
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            float top = m[j];
+            for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+                for (int r = 0; r < 16; ++r)
+                    if (t * Pr::TM + pr.wm + 32 * i + acc_row(r, g2) >= a.V)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    if (t * TM + wmi * 64 + 32 * i + acc_row(r, g2) >= a.V) acc[i][j][r] = -INFINITY;
-                    top = fmaxf(top, acc[i][j][r]);
+                        for (int j = 0; j < NI; ++j) acc[i][j][r] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            auto tile_sum = [&](float r0, float s) FA2_INLINE {
+                const float sub = r0 * LOG2E;
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(acc[i][j][r] * LOG2E - sub);
+                    asm volatile("" : "+v"(s));   // one block's exponentials at a time: all at once spill
                 }
-            const float base = top == -INFINITY ? 0.f : top;
-            l[j] *= __expf(m[j] - base);
-            m[j] = top;
+                return s;
+            };
+            float s = tile_sum(ref[j] == -INFINITY ? 0.f : ref[j], sum[j]);
+            if (__any(ref[j] == -INFINITY || !(s < 0x1p100f))) {
+                FA2_COLD_BRANCH();
+                float top = ref[j];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) l[j] += __expf(acc[i][j][r] - base);
+                    for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+                const float base = top == -INFINITY ? 0.f : top;
+                s = tile_sum(base, sum[j] * __builtin_amdgcn_exp2f((ref[j] - base) * LOG2E));
+                ref[j] = top;
+            }
+            sum[j] = s;
         }
     }
+    // Lanes, then the waves along the vocabulary (the panels are no longer read).
+    float *jm = reinterpret_cast<float *>(mem), *jl = jm + WM * Pr::TN;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        join_max_sum(m[j], l[j], __shfl_xor(m[j], 32), __shfl_xor(l[j], 32));
+    for (int j = 0; j < NI; ++j) {
+        join_max_sum(ref[j], sum[j], __shfl_xor(ref[j], 32), __shfl_xor(sum[j], 32));
         if (g2 == 0) {
-            sm[wmi][wn + 32 * j + c] = m[j];
-            sl[wmi][wn + 32 * j + c] = l[j];
+            const int at = pr.wm / (Pr::TM / WM) * Pr::TN + pr.wn + 32 * j + c;
+            jm[at] = ref[j];
+            jl[at] = sum[j];
         }
     }
     __syncthreads();
-    if (threadIdx.x < TN) {
-        float mm = sm[0][threadIdx.x], ll = sl[0][threadIdx.x];
-        join_max_sum(mm, ll, sm[1][threadIdx.x], sl[1][threadIdx.x]);
-        f2 *o = reinterpret_cast<f2 *>(a.part) + (int64_t)split * a.rows_pad + rb * TN + threadIdx.x;
-        *o = f2{mm, ll};
+    for (int i = threadIdx.x; i < Pr::TN; i += 512) {
+        float m = jm[i], l = jl[i];
+#pragma unroll
+        for (int w = 1; w < WM; ++w) join_max_sum(m, l, jm[w * Pr::TN + i], jl[w * Pr::TN + i]);
+        *(reinterpret_cast<f2 *>(a.part) + (int64_t)split * a.rows_pad + rb * Pr::TN + i) = f2{m, l};
     }
 }
 
@@ -352,100 +301,116 @@ __global__ __launch_bounds__(1024) void xent_coef_kernel(const XentArgs a) {
     }
 }
 
-// A tile of P: logits again, softmax, minus one at the target, times the row's factor.
+// A tile of P: logits again, softmax, minus one at the target, times the row's
+// factor; M side vocabulary rows, N side tokens.
 template <typename T>
-__global__ __launch_bounds__(256) void xent_p_kernel(const XentArgs a) {
-    __shared__ TileMem<T> s;
-    const int nr = a.rows_pad / TN;
+__global__ __launch_bounds__(512, 2) void xent_p_kernel(const XentArgs a) {
+    typedef Product<T, true, true, 4, 4, 2, 4> Pr;
+    __shared__ __align__(16) char mem[Pr::LDS];
+    const int nr = a.rows_pad / Pr::TN;
     const int rb = blockIdx.x % nr, vt = blockIdx.x / nr;
     const int n = a.count[0];
+    if (rb * Pr::TN >= n) return;   // no product reads these rows
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
-    const int wm = (threadIdx.x >> 6 & 1) * 64, wn = (threadIdx.x >> 7) * 64;
-    f16x acc[2][2];
-    if (rb * TN < n) {
-        const Operand<T> A = {static_cast<const T *>(a.w), a.w_stride, a.v0 + vt * TM, a.V, 0};
-        const Operand<T> B = {static_cast<const T *>(a.xc), a.dp, rb * TN, a.rows_pad, 0};
-        product_tile<T, true, true>(A, B, 0, a.dp, s, acc);
-    } else if (rb * TN >= (n + XENT_PAD - 1) / XENT_PAD * XENT_PAD) {
-        return;   // no product reads these rows
-    }
+    const int v0 = a.v0 + vt * Pr::TM;
+    Pr pr;
+    pr.init(mem);
+    pr.A.init(a.w, a.w_stride, v0, a.V, 0);
+    pr.B.init(a.xc, a.dp, rb * Pr::TN, a.rows_pad, 0);
+    f16x acc[Pr::MI][Pr::NI];
+    pr.run(0, a.dp, acc);
+    char *blk = mem + (threadIdx.x >> 6) * 4096;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int row = rb * TN + wn + 32 * j + c;
+    for (int j = 0; j < Pr::NI; ++j) {
+        const int row = rb * Pr::TN + pr.wn + 32 * j + c;
         const bool in = row < n;
-        const float lse = in ? a.lse[row] : 0.f, f = in ? a.coef[row] : 0.f;
-        const int t = in ? a.tgt[row] - a.v0 - vt * TM : -1;
+        const float f = in ? a.coef[row] : 0.f, sub = in ? a.lse[row] * LOG2E : 0.f;
+        const int t = in ? a.tgt[row] - v0 - pr.wm : -1;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < Pr::MI; ++i) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                f4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * q + e, mm = wm + 32 * i + acc_row(r, g2);
-                    const float p = __expf(acc[i][j][r] - lse) - (mm == t ? 1.f : 0.f);
-                    v[e] = in && a.v0 + vt * TM + mm < a.V && f != 0.f ? p * f : 0.f;
-                }
-                T *o = static_cast<T *>(a.P) + (int64_t)row * a.piece + vt * TM + wm + 32 * i + 8 * q + 4 * g2;
-                *reinterpret_cast<typename vec_of<T>::v4 *>(o) = __builtin_convertvector(v, typename vec_of<T>::v4);
+            for (int r = 0; r < 16; ++r) {
+                const float p = __builtin_amdgcn_exp2f(acc[i][j][r] * LOG2E - sub) * f;
+                acc[i][j][r] = f != 0.f ? p : 0.f;
             }
+            if (__any(t >= 32 * i && t < 32 * i + 32)) {
+                FA2_COLD_BRANCH();
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t == 32 * i + acc_row(r, g2)) acc[i][j][r] -= f;
+            }
+            if (v0 + pr.wm + 32 * i + 32 > a.V) {   // rows past the vocabulary
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (v0 + pr.wm + 32 * i + acc_row(r, g2) >= a.V) acc[i][j][r] = 0.f;
+            }
+        }
+        T *o = static_cast<T *>(a.P) + (int64_t)(rb * Pr::TN + pr.wn + 32 * j) * a.piece + vt * Pr::TM + pr.wm;
+#pragma unroll
+        for (int i = 0; i < Pr::MI; i += 2)
+            store_rows<T>(acc[i][j], acc[i + 1][j], 1.f, blk, o + 32 * i, a.piece, 32, 64, true);
     }
 }
 
 // dW of the piece: M side hidden columns, N side vocabulary rows, K packed tokens.
 template <typename T>
-__global__ __launch_bounds__(256) void xent_dw_kernel(const XentArgs a) {
-    __shared__ TileMem<T> s;
-    const int nd = (a.d + TM - 1) / TM;
+__global__ __launch_bounds__(512, 2) void xent_dw_kernel(const XentArgs a) {
+    typedef Product<T, false, false, 4, 4, 2, 4> Pr;
+    __shared__ __align__(16) char mem[Pr::LDS];
+    const int nd = (a.d + Pr::TM - 1) / Pr::TM;
     const int db = blockIdx.x % nd, vb = blockIdx.x / nd;
     const int n = a.count[0], kn = (n + XENT_PAD - 1) / XENT_PAD * XENT_PAD;
-    const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
-    const int wm = (threadIdx.x >> 6 & 1) * 64, wn = (threadIdx.x >> 7) * 64;
-    const Operand<T> A = {static_cast<const T *>(a.xc), a.dp, db * TM, a.dp, a.rows_pad};
-    const Operand<T> B = {static_cast<const T *>(a.P), a.piece, vb * TN, a.piece, a.rows_pad};
-    f16x acc[2][2];
-    product_tile<T, false, false>(A, B, 0, kn, s, acc);
+    Pr pr;
+    pr.init(mem);
+    pr.A.init(a.xc, a.dp, db * Pr::TM, a.dp, a.rows_pad);
+    pr.B.init(a.P, a.piece, vb * Pr::TN, a.piece, a.rows_pad);
+    f16x acc[Pr::MI][Pr::NI];
+    pr.run(0, kn, acc);
     const float u = a.unscale[0];
+    char *blk = mem + (threadIdx.x >> 6) * 4096;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int v = a.v0 + vb * TN + wn + 32 * j + c;
-        if (v >= a.v1) continue;
+    for (int j = 0; j < Pr::NI; ++j) {
+        const int v = a.v0 + vb * Pr::TN + pr.wn + 32 * j;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int col = db * TM + wm + 32 * i + acc_row(r, g2);
-                if (col < a.d) static_cast<T *>(a.dw)[(int64_t)v * a.d + col] = (T)(acc[i][j][r] * u);
-            }
+        for (int i = 0; i < Pr::MI; i += 2) {
+            const int col = db * Pr::TM + pr.wm + 32 * i;
+            store_rows<T>(acc[i][j], acc[i + 1][j], u, blk, static_cast<T *>(a.dw) + (int64_t)v * a.d + col, a.d, a.v1 - v,
+                          a.d - col, a.d % 8 == 0);
+        }
     }
 }
 
-// The piece's share of dx: M side hidden columns, N side packed tokens, K a slice
+// The piece's share of dx: M side packed tokens, N side hidden columns, K a slice
 // of the piece.
 template <typename T>
-__global__ __launch_bounds__(256) void xent_dx_kernel(const XentArgs a) {
-    __shared__ TileMem<T> s;
-    const int nd = (a.d + TM - 1) / TM, nr = a.rows_pad / TN;
+__global__ __launch_bounds__(512, 2) void xent_dx_kernel(const XentArgs a) {
+    typedef Product<T, true, false, 4, 4, 2, 4> Pr;
+    __shared__ __align__(16) char mem[Pr::LDS];
+    const int nd = (a.d + Pr::TN - 1) / Pr::TN, nr = a.rows_pad / Pr::TM;
     const int db = blockIdx.x % nd, rb = blockIdx.x / nd % nr, ks = blockIdx.x / nd / nr;
-    if (rb * TN >= a.count[0]) return;
+    if (rb * Pr::TM >= a.count[0]) return;
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
-    const int wm = (threadIdx.x >> 6 & 1) * 64, wn = (threadIdx.x >> 7) * 64;
-    const int kt = (a.v1 - a.v0 + TK - 1) / TK;
-    const int k0 = (int)((int64_t)kt * ks / a.ksplit) * TK, k1 = (int)((int64_t)kt * (ks + 1) / a.ksplit) * TK;
-    const Operand<T> A = {static_cast<const T *>(a.w) + (int64_t)a.v0 * a.w_stride, a.w_stride, db * TM, a.dp, a.V - a.v0};
-    const Operand<T> B = {static_cast<const T *>(a.P), a.piece, rb * TN, a.rows_pad, 0};
-    f16x acc[2][2];
-    product_tile<T, false, true>(A, B, k0, k1, s, acc);
+    const int kt = (a.v1 - a.v0 + PK - 1) / PK;
+    const int k0 = (int)((int64_t)kt * ks / a.ksplit) * PK, k1 = (int)((int64_t)kt * (ks + 1) / a.ksplit) * PK;
+    Pr pr;
+    pr.init(mem);
+    pr.A.init(a.P, a.piece, rb * Pr::TM, a.rows_pad, 0);
+    pr.B.init(static_cast<const T *>(a.w) + (int64_t)a.v0 * a.w_stride, a.w_stride, db * Pr::TN, a.dp, a.V - a.v0);
+    f16x acc[Pr::MI][Pr::NI];
+    pr.run(k0, k1, acc);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        float *o = a.acc + ((int64_t)ks * a.rows_pad + rb * TN + wn + 32 * j + c) * a.d;
+    for (int j = 0; j < Pr::NI; ++j) {
+        const int col = db * Pr::TN + pr.wn + 32 * j + c;
+        if (col >= a.d) continue;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < Pr::MI; ++i) {
+            float *o = a.acc + ((int64_t)ks * a.rows_pad + rb * Pr::TM + pr.wm + 32 * i) * a.d + col;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int col = db * TM + wm + 32 * i + acc_row(r, g2);
-                if (col < a.d) o[col] = a.first ? acc[i][j][r] : o[col] + acc[i][j][r];
+                float *q = o + (int64_t)acc_row(r, g2) * a.d;
+                *q = a.first ? acc[i][j][r] : *q + acc[i][j][r];
             }
+        }
     }
 }
 
@@ -474,7 +439,10 @@ __global__ __launch_bounds__(256) void xent_dx_out_kernel(const XentArgs a) {
 
 template <typename T>
 hipError_t fwd(const XentArgs &a, hipStream_t st) {
-    FA2_LAUNCH(xent_stats_kernel<T>, a.rows_pad / TN * a.splits, 256);
+    if (a.narrow)
+        FA2_LAUNCH((xent_stats_kernel<T, 1, 8, 1>), a.rows_pad / 64 * a.splits, 512);
+    else
+        FA2_LAUNCH((xent_stats_kernel<T, 4, 2, 4>), a.rows_pad / 256 * a.splits, 512);
     if (a.reduction == FA2_REDUCE_NONE && a.rows > 0)
         FA2_LAUNCH(xent_ignored_kernel, (unsigned)((a.rows + 255) / 256 < 4096 ? (a.rows + 255) / 256 : 4096), 256);
     FA2_LAUNCH(xent_join_kernel<T>, a.rows_pad / 4, 256);
@@ -484,10 +452,10 @@ hipError_t fwd(const XentArgs &a, hipStream_t st) {
 
 template <typename T>
 hipError_t piece(const XentArgs &a, hipStream_t st) {
-    const int nr = a.rows_pad / TN, nd = (a.d + TM - 1) / TM, nv = (a.v1 - a.v0 + TM - 1) / TM;
-    FA2_LAUNCH(xent_p_kernel<T>, nr * nv, 256);
-    if (a.dw) FA2_LAUNCH(xent_dw_kernel<T>, nd * nv, 256);
-    if (a.dx) FA2_LAUNCH(xent_dx_kernel<T>, nd * nr * a.ksplit, 256);
+    const int nr = a.rows_pad / 256, nd = (a.d + 255) / 256, nv = (a.v1 - a.v0 + 255) / 256;
+    FA2_LAUNCH(xent_p_kernel<T>, nr * nv, 512);
+    if (a.dw) FA2_LAUNCH(xent_dw_kernel<T>, nd * nv, 512);
+    if (a.dx) FA2_LAUNCH(xent_dx_kernel<T>, nd * nr * a.ksplit, 512);
     return hipSuccess;
 }
 

@@ -194,7 +194,7 @@ Tensor dropout(Tensor x, double p, int64_t seed) {
 // The weight as rows that the products read in place: 16-byte rows unless the
 // hidden size is padded anyway.
 Tensor weight_rows(const Tensor &w) {
-    const bool rows = w.stride(1) == 1 && w.stride(0) >= w.size(1);
+    const bool rows = w.stride(1) == 1 && w.stride(0) >= w.size(1) && w.stride(0) < (1 << 22);
     const bool fits = reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0 && w.stride(0) % 8 == 0;
     if (rows && (fits || w.size(1) % 64 != 0)) return w;
     return w.clone(at::MemoryFormat::Contiguous);
