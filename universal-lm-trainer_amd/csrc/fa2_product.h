@@ -142,26 +142,31 @@ struct Product {
         fb.init();
     }
 
-    __device__ __forceinline__ void issue(int k0, int stage) const {
-        A.issue(k0, lds + stage * STAGE);
-        B.issue(k0, lds + stage * STAGE + MP * PANEL);
+    // The stream of stages: `next` starts the transfers of the following stage, k0 of the
+    // operands, into the buffer that is free; stages are consumed in that order.
+    __device__ __forceinline__ void issue(int k0, int buf) const {
+        A.issue(k0, lds + buf * STAGE);
+        B.issue(k0, lds + buf * STAGE + MP * PANEL);
     }
 
-    __device__ __forceinline__ void compute(int stage, f16x (&acc)[MI][NI]) const {
-        typedef typename vec_of<T>::v8 v8;
-        const char *s = mem + stage * STAGE;
+    typedef typename vec_of<T>::v8 v8;
+    struct Frags {
+        v8 a[MI], b[NI];
+    };
+
+    __device__ __forceinline__ void read(Frags &f, int buf, int ks) const {
+        const char *s = mem + buf * STAGE;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            v8 a[MI], b[NI];
+        for (int i = 0; i < MI; ++i) f.a[i] = fa.read(s, wm + 32 * i, ks);
 #pragma unroll
-            for (int i = 0; i < MI; ++i) a[i] = fa.read(s, wm + 32 * i, ks);
+        for (int j = 0; j < NI; ++j) f.b[j] = fb.read(s + MP * PANEL, wn + 32 * j, ks);
+    }
+
+    static __device__ __forceinline__ void multiply(const Frags &f, f16x (&acc)[MI][NI]) {
 #pragma unroll
-            for (int j = 0; j < NI; ++j) b[j] = fb.read(s + MP * PANEL, wn + 32 * j, ks);
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NI; ++j) acc[i][j] = mfma(a[i], b[j], acc[i][j]);
-        }
+            for (int j = 0; j < NI; ++j) acc[i][j] = mfma(f.a[i], f.b[j], acc[i][j]);
     }
 
     static __device__ __forceinline__ void zero(f16x (&acc)[MI][NI]) {
@@ -171,19 +176,59 @@ struct Product {
             for (int j = 0; j < NI; ++j) acc[i][j] = zero16();
     }
 
-    // k from kbeg to kend, multiples of PK.  Leaves no transfer in flight and every
-    // wave past its last read.
-    __device__ __forceinline__ void run(int kbeg, int kend, f16x (&acc)[MI][NI]) const {
-        zero(acc);
-        if (kbeg < kend) issue(kbeg, 0);
-        int stage = 0;
-        for (int k = kbeg; k < kend; k += PK) {
+    // A stream of stages.  begin() starts the first two and reads the first
+    // fragments; steps() consumes n stages.  next(buf) starts the following stage's
+    // transfers into buffer buf, or nothing when there is none left.
+    //
+    // The fragments of each k step are read while the step before is multiplied.
+    // The one barrier of a stage stands before its last step: by then every wave
+    // holds that step's fragments, so the stage's buffer is free for the stage after
+    // the next, and the next stage has landed, so its first fragments can be read
+    // behind the last step's products.
+    Frags f0;
+    int buf;
+
+    template <typename N>
+    __device__ __forceinline__ void begin(N next) {
+        next(0);
+        next(1);
+        vm_wait<0>();
+        lds_barrier();
+        buf = 0;
+        read(f0, 0, 0);
+    }
+
+    template <typename N>
+    __device__ __forceinline__ void steps(int n, f16x (&acc)[MI][NI], N next) {
+        for (int t = 0; t < n; ++t) {
+            Frags f1;
+            read(f1, buf, 1);
+            multiply(f0, acc);
+            read(f0, buf, 2);
+            multiply(f1, acc);
+            read(f1, buf, 3);
+            multiply(f0, acc);
             vm_wait<0>();
-            lds_barrier();   // this stage has landed; every wave is done with the other
-            if (k + PK < kend) issue(k + PK, stage ^ 1);
-            compute(stage, acc);
-            stage ^= 1;
+            lds_barrier();
+            next(buf);
+            buf ^= 1;
+            read(f0, buf, 0);
+            multiply(f1, acc);
         }
+    }
+
+    // k from kbeg to kend, multiples of PK, of the operands as they are.  Leaves no
+    // transfer in flight and every wave past its last read.
+    __device__ __forceinline__ void run(int kbeg, int kend, f16x (&acc)[MI][NI]) {
+        zero(acc);
+        if (kbeg >= kend) return;
+        int k = kbeg;
+        auto next = [&](int b) FA2_INLINE {
+            if (k < kend) issue(k, b);
+            k += PK;
+        };
+        begin(next);
+        steps((kend - kbeg) / PK, acc, next);
         lds_barrier();
     }
 };

@@ -112,12 +112,15 @@ struct XentArgs {
     int g_stride;                  // none: elements between rows of g (0: one for all)
     float *coef;                   // [rows_pad]: factor of a row of P
     float *unscale;                // [1]: factor of the finished products
-    int piece;                     // vocabulary columns of a piece
-    int v0, v1;                    // the piece
-    void *P;                       // [rows_pad, piece]
-    int ksplit;                    // dX: slices of a piece, each with sums of its own
-    float *acc;                    // [ksplit, rows_pad, d]
-    bool first;                    // dX: the first piece starts the sums
+    int piece, pieces;             // vocabulary columns of a piece; pieces
+    int v0, v1;                    // the piece whose dW and dx are formed, from P
+    const void *P;                 // [rows_pad, piece]
+    int p0, p1;                    // the piece whose P is formed, into Pn
+    void *Pn;
+    int xcap;                      // dx: tiles of 256 tokens there are sums for, in all slices
+    float *acc;                    // [xcap * 256, d]
+    int wsplit;                    // dW: slices of the tokens
+    float *wacc;                   // [wsplit, piece, dp]; only with slices
     void *dx, *dw;                 // [N, d], [V, d]; null: not wanted
 };
 
@@ -125,7 +128,7 @@ hipError_t launch_xent_pack(const XentArgs &a, hipStream_t st);
 hipError_t launch_xent_fwd(const XentArgs &a, hipStream_t st);
 hipError_t launch_xent_pad_weight(const void *w, int64_t w_stride, void *out, int V, int d, int dp, int type, hipStream_t st);
 hipError_t launch_xent_bwd_prepare(const XentArgs &a, hipStream_t st);
-hipError_t launch_xent_bwd_piece(const XentArgs &a, hipStream_t st);
+hipError_t launch_xent_grad(const XentArgs &a, hipStream_t st);
 hipError_t launch_xent_bwd_finish(const XentArgs &a, hipStream_t st);
 
 hipError_t launch_norm_fwd(const NormFwdArgs &a, int x_type, int res_type, int y_type, hipStream_t st);

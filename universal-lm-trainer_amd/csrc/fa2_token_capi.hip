@@ -68,13 +68,13 @@ int check_norm_types(int x, int res, int y, bool fp8) {
 struct XentPlan {
     int rows_pad, dp;
     bool narrow;
-    int splits, piece, ksplit;
+    int splits, piece, pieces, xcap, wsplit;
     // offsets in the state
     size_t count, lse, tgt, rowmap, pos, xc, state_bytes;
     // offsets in the forward's workspace
     size_t f_weight, part, row_loss, fwd_bytes;
     // offsets in the backward's workspace
-    size_t b_weight, coef, unscale, P, acc, bwd_bytes;
+    size_t b_weight, coef, unscale, P[2], acc, wacc, bwd_bytes;
 };
 
 XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
@@ -86,11 +86,16 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     auto clamp = [](int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; };
     p.narrow = R <= 1024;
     p.splits = (int)clamp(256 / (p.narrow ? (rows + 63) / 64 : R / 256), 1, tiles);
-    // A piece's P is at most 128 MiB, half of the Infinity Cache, in equal pieces.
-    const int64_t most = clamp(((int64_t)128 << 20) / (2 * R) / XENT_PAD * XENT_PAD, XENT_PAD, 1 << 24);
-    const int64_t pieces = (V + most - 1) / most;
-    p.piece = (int)(((V + pieces - 1) / pieces + XENT_PAD - 1) / XENT_PAD * XENT_PAD);
-    p.ksplit = (int)clamp(256 / (nd * (R / 256)), 1, clamp(p.piece / 128, 1, 32));
+    // A piece's P is at most 256 MiB (twice, with more than one piece), in equal pieces.
+    const int64_t rt = R / 256, most = clamp(((int64_t)256 << 20) / (2 * R) / XENT_PAD * XENT_PAD, XENT_PAD, 1 << 24);
+    p.pieces = (int)((V + most - 1) / most);
+    p.piece = (int)(((V + p.pieces - 1) / p.pieces + XENT_PAD - 1) / XENT_PAD * XENT_PAD);
+    p.pieces = (V + p.piece - 1) / p.piece;
+    // dx: sums for all token tiles, or, when those are few, for slices up to one item a compute unit.
+    p.xcap = (int)(rt > 256 / nd ? rt : nd < 256 ? 256 / nd : 1);
+    // dW: its k, the tokens, in slices no longer than a compute unit's share of a launch (stages of 64 k).
+    const int64_t nv = p.piece / 256, share = nv * rt * (nd * 8 + (p.pieces > 1 ? p.dp / 64 + 4 : 0)) / 256;
+    p.wsplit = (int)clamp((4 * rt + share) / (share > 4 ? share + 1 : 4), 1, 16);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += up256(bytes); return o; };
     p.count = take(256);
@@ -110,8 +115,10 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     p.b_weight = take(wbytes);
     p.coef = take(R * 4);
     p.unscale = take(256);
-    p.P = take((size_t)R * p.piece * 2);
-    p.acc = take((size_t)p.ksplit * R * d * 4);
+    p.P[0] = take((size_t)R * p.piece * 2);
+    p.P[1] = p.pieces > 1 ? take((size_t)R * p.piece * 2) : p.P[0];
+    p.acc = take((size_t)p.xcap * 256 * d * 4);
+    p.wacc = take(p.wsplit > 1 ? (size_t)p.wsplit * p.piece * p.dp * 4 : 0);
     p.bwd_bytes = at;
     return p;
 }
@@ -174,7 +181,9 @@ fa2::XentArgs xent_args(const fa2_xent_params *p, const XentPlan &pl) {
     a.splits = pl.splits;
     a.narrow = pl.narrow;
     a.piece = pl.piece;
-    a.ksplit = pl.ksplit;
+    a.pieces = pl.pieces;
+    a.xcap = pl.xcap;
+    a.wsplit = pl.wsplit;
     return a;
 }
 
@@ -338,8 +347,8 @@ int fa2_xent_bwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
     a.g_stride = (int)p->dloss_stride;
     a.coef = reinterpret_cast<float *>(w + pl.coef);
     a.unscale = reinterpret_cast<float *>(w + pl.unscale);
-    a.P = w + pl.P;
     a.acc = reinterpret_cast<float *>(w + pl.acc);
+    a.wacc = reinterpret_cast<float *>(w + pl.wacc);
     a.dx = p->rows > 0 ? p->dx : nullptr;
     a.dw = p->dweight;
     hipError_t e = hipSuccess;
@@ -349,11 +358,15 @@ int fa2_xent_bwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
         a.w_stride = a.dp;
     }
     if (e == hipSuccess) e = fa2::launch_xent_bwd_prepare(a, st);
-    for (int v0 = 0; v0 < a.V && e == hipSuccess; v0 += a.piece) {
-        a.v0 = v0;
-        a.v1 = a.V - v0 < a.piece ? a.V : v0 + a.piece;
-        a.first = v0 == 0;
-        e = fa2::launch_xent_bwd_piece(a, st);
+    for (int i = 0; i <= a.pieces && e == hipSuccess; ++i) {   // P of piece i beside the gradients of piece i - 1
+        auto edge = [&](int k) { return (int64_t)k * a.piece < a.V ? k * a.piece : a.V; };
+        a.v0 = i > 0 ? edge(i - 1) : 0;
+        a.v1 = i > 0 ? edge(i) : 0;
+        a.p0 = edge(i);
+        a.p1 = edge(i + 1);
+        a.P = w + pl.P[(i + 1) & 1];
+        a.Pn = w + pl.P[i & 1];
+        e = fa2::launch_xent_grad(a, st);
     }
     if (e == hipSuccess && a.dx) e = fa2::launch_xent_bwd_finish(a, st);
     return launched("cross entropy backward", e);

@@ -10,7 +10,8 @@
 // second kernel joins.  Backward, for one piece of the vocabulary after another:
 // the piece's logits again, turned into P = factor * G and rounded to the
 // operands' type in a scratch of [tokens, piece]; then dW of the piece's rows,
-// which is complete, and the piece's share of dx, summed in fp32.
+// which is complete, and the piece's share of dx, summed in fp32.  P of the next
+// piece goes beside dW and dx of this one, into a second scratch.
 //
 // Tokens that do not count are taken out first (packed rows), so that no product
 // works on them and nothing in their states, inf and NaN included, reaches a result.
@@ -20,6 +21,8 @@
 // the matrix units; the gradients themselves are rounded to the same type.  P is
 // scaled so that its largest possible value is 2^15: in fp16 probabilities down
 // to 2^-29 stay normal numbers.
+#include <type_traits>
+
 #include "fa2_product.h"
 
 namespace fa2 {
@@ -115,7 +118,9 @@ __device__ __forceinline__ void join_max_sum(float &m, float &l, float m2, float
 // M side are vocabulary rows, the N side tokens: a lane holds one token's logits.
 // Each lane keeps a reference r and the sum of exp(z - r) of the logits it has
 // seen.  r is the maximum of the lane's first tile and moves only when a sum
-// passes 2^100: fp32 holds the terms of any larger logits until then.
+// passes 2^100: fp32 holds the terms of any larger logits until then.  The slice's
+// tiles are one stream of stages: the next tile's transfers run behind the
+// exponentials.
 template <typename T, int NP, int WM, int WN>
 __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
     typedef Product<T, true, true, 4, NP, WM, WN> Pr;
@@ -129,6 +134,7 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
     Pr pr;
     pr.init(mem);
+    pr.A.init(a.w, a.w_stride, t0 * Pr::TM, a.V, 0);
     pr.B.init(a.xc, a.dp, rb * Pr::TN, a.rows_pad, 0);
     float ref[NI], sum[NI];
 #pragma unroll
@@ -136,27 +142,35 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
         ref[j] = -INFINITY;
         sum[j] = 0.f;
     }
+    int nt = t0, nk = 0;   // tile and k of the next stage
+    auto next = [&](int buf) FA2_INLINE {
+        if (nt >= t1) return;
+        pr.issue(nk, buf);
+        nk += PK;
+        if (nk == a.dp) {
+            nk = 0;
+            if (++nt < t1) pr.A.init(a.w, a.w_stride, nt * Pr::TM, a.V, 0);
+        }
+    };
+    pr.begin(next);
     for (int t = t0; t < t1; ++t) {
         f16x acc[MI][NI];
-        pr.A.init(a.w, a.w_stride, t * Pr::TM, a.V, 0);
-        pr.run(0, a.dp, acc);
-        if ((t + 1) * Pr::TM > a.V) {   // rows past the vocabulary
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (t * Pr::TM + pr.wm + 32 * i + acc_row(r, g2) >= a.V)
-#pragma unroll
-                        for (int j = 0; j < NI; ++j) acc[i][j][r] = -INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < NI; ++j) {
+        pr.zero(acc);
+        pr.steps(a.dp / PK, acc, next);
+        // Rows of this wave's part that are past the vocabulary (in the last tile) are left out.
+        const int left = a.V - t * Pr::TM - pr.wm;
+        auto add_tile = [&](auto tail, int j) FA2_INLINE {
+            constexpr bool TAIL = decltype(tail)::value;
+            auto in = [&](int i, int r) FA2_INLINE { return !TAIL || 32 * i + acc_row(r, g2) < left; };
             auto tile_sum = [&](float r0, float s) FA2_INLINE {
                 const float sub = r0 * LOG2E;
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(acc[i][j][r] * LOG2E - sub);
+                    for (int r = 0; r < 16; ++r) {
+                        const float e = __builtin_amdgcn_exp2f(acc[i][j][r] * LOG2E - sub);
+                        s += in(i, r) ? e : 0.f;
+                    }
                     asm volatile("" : "+v"(s));   // one block's exponentials at a time: all at once spill
                 }
                 return s;
@@ -168,14 +182,23 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+                    for (int r = 0; r < 16; ++r) top = in(i, r) ? fmaxf(top, acc[i][j][r]) : top;
                 const float base = top == -INFINITY ? 0.f : top;
                 s = tile_sum(base, sum[j] * __builtin_amdgcn_exp2f((ref[j] - base) * LOG2E));
                 ref[j] = top;
             }
             sum[j] = s;
+        };
+        if (left >= Pr::TM / WM) {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) add_tile(std::false_type(), j);
+        } else {
+            FA2_COLD_BRANCH();
+#pragma unroll
+            for (int j = 0; j < NI; ++j) add_tile(std::true_type(), j);
         }
     }
+    lds_barrier();
     // Lanes, then the waves along the vocabulary (the panels are no longer read).
     float *jm = reinterpret_cast<float *>(mem), *jl = jm + WM * Pr::TN;
 #pragma unroll
@@ -301,116 +324,217 @@ __global__ __launch_bounds__(1024) void xent_coef_kernel(const XentArgs a) {
     }
 }
 
-// A tile of P: logits again, softmax, minus one at the target, times the row's
+// The work of one launch of the backward: dW and dx of a piece, and P of the piece
+// after it, as items of one grid, the long ones first; P's many short items fill the
+// compute units that the others leave.  Lengths are in stages of 64 k.
+struct XentWork {
+    int rt;            // tiles of 256 tokens that count
+    int dw, dx, p;     // items
+    int xs;            // slices of dx's k
+};
+
+constexpr int P_STRIP = 4;       // tiles of P an item
+constexpr int P_TILE_EXTRA = 4;  // stages that the softmax of a tile of P takes as long as
+
+__device__ __forceinline__ XentWork xent_work(const XentArgs &a, int n) {
+    XentWork k;
+    const int nd = (a.d + 255) / 256, nv = (a.v1 - a.v0 + 255) / 256, nvp = (a.p1 - a.p0 + 255) / 256;
+    k.rt = (n + 255) / 256;
+    // Slices of dx: no longer than three quarters of a compute unit's share of a
+    // launch (with pieces of full width; the same number for every piece).
+    const int64_t full = a.piece / 256;
+    const int64_t total = full * k.rt * (nd * 8 + (a.pieces > 1 ? a.dp / PK + P_TILE_EXTRA : 0));
+    const int share = (int)max((int64_t)4, total * 3 / (4 * 256));
+    k.xs = max(1, min((a.piece / PK + share - 1) / share, a.xcap / max(k.rt, 1)));
+    k.dw = a.dw ? nd * nv * a.wsplit : 0;
+    k.dx = a.dx && nv > 0 ? nd * k.rt * k.xs : 0;
+    k.p = k.rt * ((nvp + P_STRIP - 1) / P_STRIP);
+    return k;
+}
+
+// Workgroups go to the eight XCDs in turn: the l-th of n items, numbered so that an
+// XCD's items are neighbours (their operands meet in its L2).
+__device__ __forceinline__ int xcd_item(int l, int n) {
+    const int x = l & 7;
+    return x * (n >> 3) + min(x, n & 7) + (l >> 3);
+}
+
+// P_STRIP tiles of P: logits again, softmax, minus one at the target, times the row's
 // factor; M side vocabulary rows, N side tokens.
 template <typename T>
-__global__ __launch_bounds__(512, 2) void xent_p_kernel(const XentArgs a) {
+__device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k, int item, int n, char *mem, char *out) {
     typedef Product<T, true, true, 4, 4, 2, 4> Pr;
-    __shared__ __align__(16) char mem[Pr::LDS];
-    const int nr = a.rows_pad / Pr::TN;
-    const int rb = blockIdx.x % nr, vt = blockIdx.x / nr;
-    const int n = a.count[0];
-    if (rb * Pr::TN >= n) return;   // no product reads these rows
+    const int tiles = (a.p1 - a.p0 + 255) / 256, strips = (tiles + P_STRIP - 1) / P_STRIP;
+    // groups of 8 token tiles, in a group the tokens fastest
+    const int g = item / (8 * strips), gs = min(8, k.rt - 8 * g), in = item - g * 8 * strips;
+    const int rb = 8 * g + in % gs, t0 = in / gs * P_STRIP, t1 = min(tiles, t0 + P_STRIP);
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
-    const int v0 = a.v0 + vt * Pr::TM;
     Pr pr;
     pr.init(mem);
-    pr.A.init(a.w, a.w_stride, v0, a.V, 0);
+    pr.A.init(a.w, a.w_stride, a.p0 + t0 * Pr::TM, a.V, 0);
     pr.B.init(a.xc, a.dp, rb * Pr::TN, a.rows_pad, 0);
-    f16x acc[Pr::MI][Pr::NI];
-    pr.run(0, a.dp, acc);
-    char *blk = mem + (threadIdx.x >> 6) * 4096;
+    float f[Pr::NI], sub[Pr::NI];
+    int tgt[Pr::NI];
 #pragma unroll
     for (int j = 0; j < Pr::NI; ++j) {
         const int row = rb * Pr::TN + pr.wn + 32 * j + c;
-        const bool in = row < n;
-        const float f = in ? a.coef[row] : 0.f, sub = in ? a.lse[row] * LOG2E : 0.f;
-        const int t = in ? a.tgt[row] - v0 - pr.wm : -1;
+        f[j] = a.coef[row];
+        sub[j] = row < n ? a.lse[row] * LOG2E : 0.f;
+        tgt[j] = a.tgt[row] - pr.wm;
+    }
+    int nt = t0, nk = 0;
+    auto next = [&](int buf) FA2_INLINE {
+        if (nt >= t1) return;
+        pr.issue(nk, buf);
+        nk += PK;
+        if (nk == a.dp) {
+            nk = 0;
+            if (++nt < t1) pr.A.init(a.w, a.w_stride, a.p0 + nt * Pr::TM, a.V, 0);
+        }
+    };
+    pr.begin(next);
+    char *blk = out + (threadIdx.x >> 6) * 4096;
+    for (int t = t0; t < t1; ++t) {
+        const int v0 = a.p0 + t * Pr::TM;
+        f16x acc[Pr::MI][Pr::NI];
+        pr.zero(acc);
+        pr.steps(a.dp / PK, acc, next);
 #pragma unroll
-        for (int i = 0; i < Pr::MI; ++i) {
+        for (int j = 0; j < Pr::NI; ++j) {
+            T *o = static_cast<T *>(a.Pn) + (int64_t)(rb * Pr::TN + pr.wn + 32 * j) * a.piece + t * Pr::TM + pr.wm;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(acc[i][j][r] * LOG2E - sub) * f;
-                acc[i][j][r] = f != 0.f ? p : 0.f;
-            }
-            if (__any(t >= 32 * i && t < 32 * i + 32)) {
-                FA2_COLD_BRANCH();
+            for (int i = 0; i < Pr::MI; i += 2) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (t == 32 * i + acc_row(r, g2)) acc[i][j][r] -= f;
-            }
-            if (v0 + pr.wm + 32 * i + 32 > a.V) {   // rows past the vocabulary
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (v0 + pr.wm + 32 * i + acc_row(r, g2) >= a.V) acc[i][j][r] = 0.f;
+                    for (int r = 0; r < 16; ++r) {
+                        const float p = __builtin_amdgcn_exp2f(acc[i + h][j][r] * LOG2E - sub[j]) * f[j];
+                        acc[i + h][j][r] = f[j] != 0.f ? p : 0.f;
+                    }
+                    const int at = tgt[j] - v0 - 32 * (i + h);
+                    if (__any(at >= 0 && at < 32)) {
+                        FA2_COLD_BRANCH();
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (at == acc_row(r, g2)) acc[i + h][j][r] -= f[j];
+                    }
+                    if (v0 + pr.wm + 32 * (i + h) + 32 > a.V) {   // rows past the vocabulary
+                        FA2_COLD_BRANCH();
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (v0 + pr.wm + 32 * (i + h) + acc_row(r, g2) >= a.V) acc[i + h][j][r] = 0.f;
+                    }
+                }
+                store_rows<T>(acc[i][j], acc[i + 1][j], 1.f, blk, o + 32 * i, a.piece, 32, 64, true);
             }
         }
-        T *o = static_cast<T *>(a.P) + (int64_t)(rb * Pr::TN + pr.wn + 32 * j) * a.piece + vt * Pr::TM + pr.wm;
-#pragma unroll
-        for (int i = 0; i < Pr::MI; i += 2)
-            store_rows<T>(acc[i][j], acc[i + 1][j], 1.f, blk, o + 32 * i, a.piece, 32, 64, true);
     }
 }
 
-// dW of the piece: M side hidden columns, N side vocabulary rows, K packed tokens.
+// A tile of the piece's dW, or of a slice of its k: M side hidden columns, N side
+// vocabulary rows, K packed tokens.
 template <typename T>
-__global__ __launch_bounds__(512, 2) void xent_dw_kernel(const XentArgs a) {
+__device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n, char *mem) {
     typedef Product<T, false, false, 4, 4, 2, 4> Pr;
-    __shared__ __align__(16) char mem[Pr::LDS];
-    const int nd = (a.d + Pr::TM - 1) / Pr::TM;
-    const int db = blockIdx.x % nd, vb = blockIdx.x / nd;
-    const int n = a.count[0], kn = (n + XENT_PAD - 1) / XENT_PAD * XENT_PAD;
+    const int nd = (a.d + 255) / 256, nv = (a.v1 - a.v0 + 255) / 256;
+    const int db = item % nd, vb = item / nd % nv, s = item / nd / nv;
+    const int kt = (n + 255) / 256 * (256 / PK);
+    const int k0 = (int)((int64_t)kt * s / a.wsplit) * PK, k1 = (int)((int64_t)kt * (s + 1) / a.wsplit) * PK;
     Pr pr;
     pr.init(mem);
     pr.A.init(a.xc, a.dp, db * Pr::TM, a.dp, a.rows_pad);
     pr.B.init(a.P, a.piece, vb * Pr::TN, a.piece, a.rows_pad);
     f16x acc[Pr::MI][Pr::NI];
-    pr.run(0, kn, acc);
+    pr.run(k0, k1, acc);
+    const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
     const float u = a.unscale[0];
     char *blk = mem + (threadIdx.x >> 6) * 4096;
 #pragma unroll
     for (int j = 0; j < Pr::NI; ++j) {
-        const int v = a.v0 + vb * Pr::TN + pr.wn + 32 * j;
+        const int v = vb * Pr::TN + pr.wn + 32 * j;   // of the piece
 #pragma unroll
         for (int i = 0; i < Pr::MI; i += 2) {
             const int col = db * Pr::TM + pr.wm + 32 * i;
-            store_rows<T>(acc[i][j], acc[i + 1][j], u, blk, static_cast<T *>(a.dw) + (int64_t)v * a.d + col, a.d, a.v1 - v,
-                          a.d - col, a.d % 8 == 0);
+            if (a.wsplit == 1) {
+                store_rows<T>(acc[i][j], acc[i + 1][j], u, blk, static_cast<T *>(a.dw) + (int64_t)(a.v0 + v) * a.d + col, a.d,
+                              a.v1 - a.v0 - v, a.d - col, a.d % 8 == 0);
+            } else {   // rows of the slice's sums: [wsplit][piece][dp], four columns a store
+                float *o = a.wacc + ((int64_t)s * a.piece + v + c) * a.dp + col;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (col + 32 * h < a.dp) {
+                            f4 x;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] = acc[i + h][j][4 * q + e];
+                            *reinterpret_cast<f4 *>(o + 32 * h + 8 * q + 4 * g2) = x;
+                        }
+            }
         }
     }
 }
 
-// The piece's share of dx: M side packed tokens, N side hidden columns, K a slice
-// of the piece.
+// A tile of the piece's share of dx, or of a slice of its k: M side packed tokens, N
+// side hidden columns, K the piece.
 template <typename T>
-__global__ __launch_bounds__(512, 2) void xent_dx_kernel(const XentArgs a) {
+__device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &k, int item, char *mem) {
     typedef Product<T, true, false, 4, 4, 2, 4> Pr;
-    __shared__ __align__(16) char mem[Pr::LDS];
-    const int nd = (a.d + Pr::TN - 1) / Pr::TN, nr = a.rows_pad / Pr::TM;
-    const int db = blockIdx.x % nd, rb = blockIdx.x / nd % nr, ks = blockIdx.x / nd / nr;
-    if (rb * Pr::TM >= a.count[0]) return;
-    const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
+    const int nd = (a.d + 255) / 256;
+    const int db = item % nd, rb = item / nd % k.rt, s = item / nd / k.rt;
     const int kt = (a.v1 - a.v0 + PK - 1) / PK;
-    const int k0 = (int)((int64_t)kt * ks / a.ksplit) * PK, k1 = (int)((int64_t)kt * (ks + 1) / a.ksplit) * PK;
+    const int k0 = (int)((int64_t)kt * s / k.xs) * PK, k1 = (int)((int64_t)kt * (s + 1) / k.xs) * PK;
     Pr pr;
     pr.init(mem);
     pr.A.init(a.P, a.piece, rb * Pr::TM, a.rows_pad, 0);
     pr.B.init(static_cast<const T *>(a.w) + (int64_t)a.v0 * a.w_stride, a.w_stride, db * Pr::TN, a.dp, a.V - a.v0);
     f16x acc[Pr::MI][Pr::NI];
     pr.run(k0, k1, acc);
+    const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
 #pragma unroll
     for (int j = 0; j < Pr::NI; ++j) {
         const int col = db * Pr::TN + pr.wn + 32 * j + c;
         if (col >= a.d) continue;
 #pragma unroll
         for (int i = 0; i < Pr::MI; ++i) {
-            float *o = a.acc + ((int64_t)ks * a.rows_pad + rb * Pr::TM + pr.wm + 32 * i) * a.d + col;
+            float *o = a.acc + ((int64_t)(s * k.rt + rb) * Pr::TM + pr.wm + 32 * i) * a.d + col;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 float *q = o + (int64_t)acc_row(r, g2) * a.d;
-                *q = a.first ? acc[i][j][r] : *q + acc[i][j][r];
+                *q = a.v0 == 0 ? acc[i][j][r] : *q + acc[i][j][r];
             }
         }
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(512, 2) void xent_grad_kernel(const XentArgs a) {
+    constexpr int PANELS = Product<T, true, true, 4, 4, 2, 4>::LDS;
+    __shared__ __align__(16) char mem[PANELS + 8 * 4096];
+    const int n = a.count[0];
+    const XentWork k = xent_work(a, n);
+    int l = blockIdx.x;
+    const bool dw_first = (int64_t)k.rt * 4 * k.xs * PK > (int64_t)(a.v1 - a.v0) * a.wsplit;   // the longer ones
+    if (dw_first && l < k.dw) return xent_dw_item<T>(a, xcd_item(l, k.dw), n, mem);
+    l -= dw_first ? k.dw : 0;
+    if (l < k.dx) return xent_dx_item<T>(a, k, xcd_item(l, k.dx), mem);
+    l -= k.dx;
+    if (!dw_first && l < k.dw) return xent_dw_item<T>(a, xcd_item(l, k.dw), n, mem);
+    l -= dw_first ? 0 : k.dw;
+    if (l < k.p) xent_p_item<T>(a, k, xcd_item(l, k.p), n, mem, mem + PANELS);
+}
+
+// dW of a piece whose k was sliced: the slices' sums in order.
+template <typename T>
+__global__ __launch_bounds__(256) void xent_dw_join_kernel(const XentArgs a) {
+    const float u = a.unscale[0];
+    const int64_t total = (int64_t)(a.v1 - a.v0) * a.d;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+        const int64_t v = e / a.d;
+        const int c = (int)(e - v * a.d);
+        float x = 0.f;
+        for (int s = 0; s < a.wsplit; ++s) x += a.wacc[((int64_t)s * a.piece + v) * a.dp + c];
+        static_cast<T *>(a.dw)[(int64_t)a.v0 * a.d + e] = (T)(x * u);
     }
 }
 
@@ -418,12 +542,13 @@ __global__ __launch_bounds__(512, 2) void xent_dx_kernel(const XentArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void xent_dx_out_kernel(const XentArgs a) {
     const int64_t total = a.rows * a.d;
+    const XentWork k = xent_work(a, a.count[0]);
     for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
         const int64_t i = e / a.d;
         const int c = (int)(e - i * a.d), j = a.pos[i];
         float v = 0.f;
         if (j >= 0) {
-            for (int s = 0; s < a.ksplit; ++s) v += a.acc[((int64_t)s * a.rows_pad + j) * a.d + c];
+            for (int s = 0; s < k.xs; ++s) v += a.acc[((int64_t)s * k.rt * 256 + j) * a.d + c];
             v *= a.unscale[0];
         }
         static_cast<T *>(a.dx)[e] = (T)v;
@@ -450,12 +575,16 @@ hipError_t fwd(const XentArgs &a, hipStream_t st) {
     return hipSuccess;
 }
 
+// P of [p0, p1) beside dW and dx of [v0, v1); either may be empty.
 template <typename T>
-hipError_t piece(const XentArgs &a, hipStream_t st) {
-    const int nr = a.rows_pad / 256, nd = (a.d + 255) / 256, nv = (a.v1 - a.v0 + 255) / 256;
-    FA2_LAUNCH(xent_p_kernel<T>, nr * nv, 512);
-    if (a.dw) FA2_LAUNCH(xent_dw_kernel<T>, nd * nv, 512);
-    if (a.dx) FA2_LAUNCH(xent_dx_kernel<T>, nd * nr * a.ksplit, 512);
+hipError_t grad(const XentArgs &a, hipStream_t st) {
+    const int rt = a.rows_pad / 256, nd = (a.d + 255) / 256, nv = (a.v1 - a.v0 + 255) / 256, np = (a.p1 - a.p0 + 255) / 256;
+    const int items = nd * nv * a.wsplit + (nv ? nd * a.xcap : 0) + rt * ((np + P_STRIP - 1) / P_STRIP);   // the most there can be
+    FA2_LAUNCH(xent_grad_kernel<T>, items, 512);
+    if (nv && a.dw && a.wsplit > 1) {
+        const int64_t want = ((int64_t)(a.v1 - a.v0) * a.d + 255) / 256;
+        FA2_LAUNCH(xent_dw_join_kernel<T>, (unsigned)(want < 8192 ? want : 8192), 256);
+    }
     return hipSuccess;
 }
 
@@ -490,8 +619,8 @@ hipError_t launch_xent_bwd_prepare(const XentArgs &a, hipStream_t st) {
     return hipSuccess;
 }
 
-hipError_t launch_xent_bwd_piece(const XentArgs &a, hipStream_t st) {
-    return a.type == FA2_F16 ? piece<_Float16>(a, st) : piece<__bf16>(a, st);
+hipError_t launch_xent_grad(const XentArgs &a, hipStream_t st) {
+    return a.type == FA2_F16 ? grad<_Float16>(a, st) : grad<__bf16>(a, st);
 }
 
 hipError_t launch_xent_bwd_finish(const XentArgs &a, hipStream_t st) {
