@@ -176,6 +176,19 @@ struct Product {
             for (int j = 0; j < NI; ++j) acc[i][j] = zero16();
     }
 
+    // Holds the scheduler to the order of a k step: its products, with the reads of the
+    // next step's fragments spread over the first of them (left to itself it moves the
+    // reads to their use, and every step waits for LDS).
+    static __device__ __forceinline__ void interleave() {
+        constexpr int R = MI * (AROWS ? 1 : 2) + NI * (BROWS ? 1 : 2), M = MI * NI;
+        constexpr int PER = (R + M - 1) / M;   // reads a product
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            if (i * PER < R) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);   // LDS reads
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                      // MFMA
+        }
+    }
+
     // A stream of stages.  begin() starts the first two and reads the first
     // fragments; steps() consumes n stages.  next(buf) starts the following stage's
     // transfers into buffer buf, or nothing when there is none left.
@@ -204,16 +217,20 @@ struct Product {
             Frags f1;
             read(f1, buf, 1);
             multiply(f0, acc);
+            interleave();
             read(f0, buf, 2);
             multiply(f1, acc);
+            interleave();
             read(f1, buf, 3);
             multiply(f0, acc);
+            interleave();
             vm_wait<0>();
             lds_barrier();
             next(buf);
             buf ^= 1;
             read(f0, buf, 0);
             multiply(f1, acc);
+            interleave();
         }
     }
 

@@ -162,20 +162,20 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
         auto add_tile = [&](auto tail, int j) FA2_INLINE {
             constexpr bool TAIL = decltype(tail)::value;
             auto in = [&](int i, int r) FA2_INLINE { return !TAIL || 32 * i + acc_row(r, g2) < left; };
-            auto tile_sum = [&](float r0, float s) FA2_INLINE {
-                const float sub = r0 * LOG2E;
+            auto tile_sum = [&](float r0, float s, float log2e) FA2_INLINE {
+                const float sub = r0 * log2e;
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const float e = __builtin_amdgcn_exp2f(acc[i][j][r] * LOG2E - sub);
+                        const float e = __builtin_amdgcn_exp2f(acc[i][j][r] * log2e - sub);
                         s += in(i, r) ? e : 0.f;
                     }
                     asm volatile("" : "+v"(s));   // one block's exponentials at a time: all at once spill
                 }
                 return s;
             };
-            float s = tile_sum(ref[j] == -INFINITY ? 0.f : ref[j], sum[j]);
+            float s = tile_sum(ref[j] == -INFINITY ? 0.f : ref[j], sum[j], LOG2E);
             if (__any(ref[j] == -INFINITY || !(s < 0x1p100f))) {
                 FA2_COLD_BRANCH();
                 float top = ref[j];
@@ -184,7 +184,9 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) top = in(i, r) ? fmaxf(top, acc[i][j][r]) : top;
                 const float base = top == -INFINITY ? 0.f : top;
-                s = tile_sum(base, sum[j] * __builtin_amdgcn_exp2f((ref[j] - base) * LOG2E));
+                float log2e = LOG2E;
+                asm volatile("" : "+v"(log2e));   // keeps the first sum's products from being held for this one
+                s = tile_sum(base, sum[j] * __builtin_amdgcn_exp2f((ref[j] - base) * LOG2E), log2e);
                 ref[j] = top;
             }
             sum[j] = s;
