@@ -126,12 +126,12 @@ def test_cross_entropy_memory_is_bounded(rows, d, V):
     dp = (d + 63) // 64 * 64
     copy = V * dp * 2 if d % 64 else 0
     assert lib.fa2_xent_state_bytes(rows, d) <= pad * (dp * 2 + 16) + rows * 4 + 4096
-    # partial sums: at most 1024 slices of a 128-row block, or one a token
-    assert lib.fa2_xent_fwd_workspace_bytes(rows, d, V) <= copy + 8 * max(1024 * 256, pad) + 4 * pad + 8192
+    # partial results of at most 1024 workgroups of 256 tokens, or one a token
+    assert lib.fa2_xent_fwd_workspace_bytes(rows, d, V) <= copy + 8 * max(1024 * 256, pad) + 8 * pad + 8192
     # two pieces of at most 256 MiB (or of their least width, 256 columns), fp32 sums of dx for every token or
-    # one item a compute unit, and of at most 16 slices of dW where tokens are many and the vocabulary is small
+    # one item a slot, and of at most 16 slices of dW where tokens are many and the vocabulary is small
     piece = 2 * (max(256 << 20, pad * 512) + 512 * pad)
-    slices = 4 * max(pad, 256 * 256) * d + 16 * 4 * dp * min((V + 255) // 256 * 256, max(256, (256 << 20) // (2 * pad) + 256))
+    slices = 4 * max(pad, 256 * 256) * dp + 16 * 4 * dp * min((V + 255) // 256 * 256, max(256, (256 << 20) // (2 * pad) + 256))
     assert lib.fa2_xent_bwd_workspace_bytes(rows, d, V) <= copy + piece + 4 * pad + slices + 8192
 
 

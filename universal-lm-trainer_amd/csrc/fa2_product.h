@@ -25,31 +25,32 @@ constexpr int PANEL = 8192;    // bytes
 constexpr int PK = 64;         // k of a stage
 
 // One operand of a tile: where the transfers of this thread read.  Eight waves
-// move a panel, wave w its rows 8 w .. 8 w + 7.
-template <bool ROWS, int NP>
+// move a panel, wave w its rows 8 w .. 8 w + 7.  PADDED (ROWS): the matrix has every row of
+// the tile.
+template <bool ROWS, bool PADDED, int NP>
 struct Feed {
     uint64_t base;                 // ROWS: first row, k = 0; else k = 0, column 0
-    uint32_t ld;                   // bytes of a row
-    uint32_t off[ROWS ? NP : 1];   // this lane's bytes from base (ROWS: in each panel)
-    uint32_t col[ROWS ? 1 : NP];   // else: bytes of each panel's first column
-    int kleft;                     // else: k rows there are
+    uint32_t ld;                   // bytes of a row, below 2^24
+    uint32_t row, chunk;           // this lane's row of a panel; byte in the row
+    int last;                      // last row there is (k row, if not ROWS), from base
+    uint32_t col[ROWS ? 1 : NP];   // not ROWS: bytes of each panel's first column
 
     // p: the matrix; first: the tile's first row (column); limit: rows (columns, a
     // multiple of 64) there are, at least 1 (64); k rows klimit.  What lies past a limit is
     // read from the last row or panel there is.
     __device__ __forceinline__ void init(const void *p, int64_t ld_elems, int first, int limit, int klimit) {
-        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = 8 * w + (lane >> 3);
+        const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        row = 8 * w + (lane >> 3);
         ld = (uint32_t)ld_elems * 2;
         if constexpr (ROWS) {
             const int f0 = min(first, limit - 1);
             base = uniform((uint64_t)(uintptr_t)p + (uint64_t)f0 * (uint64_t)ld);
-            const uint32_t ch = (uint32_t)((lane & 7) ^ swz_rows(r)) << 4;
-#pragma unroll
-            for (int j = 0; j < NP; ++j) off[j] = (uint32_t)min(64 * j + r, limit - 1 - f0) * ld + ch;
+            last = limit - 1 - f0;
+            chunk = (uint32_t)((lane & 7) ^ swz_rows(row)) << 4;
         } else {
             base = uniform((uint64_t)(uintptr_t)p);
-            off[0] = (uint32_t)((lane & 7) ^ swz_tr(r)) << 4;
-            kleft = klimit;
+            last = klimit - 1;
+            chunk = (uint32_t)((lane & 7) ^ swz_tr(row)) << 4;
 #pragma unroll
             for (int j = 0; j < NP; ++j) col[j] = (uint32_t)min(first + 64 * j, limit - 64) * 2;
         }
@@ -61,16 +62,24 @@ struct Feed {
         return ((uint64_t)hi << 32) | lo;
     }
 
-    // Starts the transfers of stage k0 / PK into the panels at LDS address `lds`.
+    // Starts the transfers of stage k0 / PK into the panels at LDS address `lds`.  Rows are
+    // held to the last one at every issue: offsets kept for each panel cost the registers
+    // that make the forward's kernel reload some from scratch memory, behind the
+    // transfers in flight.
     __device__ __forceinline__ void issue(int k0, uint32_t lds) const {
-        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        lds += w * 1024;
+        lds += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
         if constexpr (ROWS) {
+            const uint64_t b = base + (uint64_t)(uint32_t)k0 * 2;
+            int r = (int)row;
+            if (!PADDED) asm volatile("" : "+v"(r));   // no offset leaves the loop
 #pragma unroll
-            for (int j = 0; j < NP; ++j) lds_dma16_at(base + (uint64_t)(uint32_t)k0 * 2, off[j], lds + j * PANEL);
+            for (int j = 0; j < NP; ++j)
+                if (PADDED)
+                    lds_dma16_at(b + (uint64_t)(64 * j) * ld, mul_u24(ld, (uint32_t)r) + chunk, lds + j * PANEL);
+                else
+                    lds_dma16_at(b, mul_u24(ld, (uint32_t)min(64 * j + r, last)) + chunk, lds + j * PANEL);
         } else {
-            const int r = 8 * (threadIdx.x >> 6) + ((threadIdx.x & 63) >> 3);
-            const uint32_t o = (uint32_t)min(r, kleft - 1 - k0) * ld + off[0];
+            const uint32_t o = mul_u24(ld, (uint32_t)min((int)row, last - k0)) + chunk;
             const uint64_t b = base + (uint64_t)(uint32_t)k0 * ld;
 #pragma unroll
             for (int j = 0; j < NP; ++j) lds_dma16_at(b + col[j], o, lds + j * PANEL);
@@ -116,7 +125,8 @@ struct Frag {
 };
 
 // Tile of 64 MP x 64 NP by eight waves in WM x WN, each (64 MP / WM) x (64 NP / WN).
-template <typename T, bool AROWS, bool BROWS, int MP, int NP, int WM, int WN>
+// APADDED: A has every row of the tile (B always has).
+template <typename T, bool AROWS, bool BROWS, bool APADDED, int MP, int NP, int WM, int WN>
 struct Product {
     static_assert(WM * WN == 8, "eight waves");
     static constexpr int TM = 64 * MP, TN = 64 * NP;
@@ -124,8 +134,8 @@ struct Product {
     static constexpr int STAGE = (MP + NP) * PANEL;
     static constexpr int LDS = 2 * STAGE;
 
-    Feed<AROWS, MP> A;
-    Feed<BROWS, NP> B;
+    Feed<AROWS, APADDED, MP> A;
+    Feed<BROWS, true, NP> B;
     Frag<T, AROWS> fa;
     Frag<T, BROWS> fb;
     char *mem;

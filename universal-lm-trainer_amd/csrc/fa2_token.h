@@ -80,6 +80,7 @@ struct DropoutArgs {
 // are `rows_pad` (a multiple of XENT_PAD) with zeros behind the last one.
 constexpr int XENT_PAD = 256;      // packed rows and a piece's columns: multiples of this
 constexpr int XENT_KPAD = 64;      // the hidden size the products see: a multiple of this
+constexpr int XENT_NARROW_V = 128; // vocabulary rows of the forward's tiles of 64 tokens
 
 struct XentArgs {
     int64_t rows;                  // N
@@ -95,36 +96,39 @@ struct XentArgs {
     int64_t ignore;
     int reduction;
     // kept for the backward
-    int *count;                    // [0]: rows that count
+    int *count;                    // tokens that count, slices of the forward
     int *pos;                      // [N]: packed row of a token, -1 where ignored
     int *rowmap;                   // [rows_pad]
     int *tgt;                      // [rows_pad]: target, -1 where it is outside the vocabulary
     float *lse;                    // [rows_pad]
     void *xc;                      // [rows_pad, dp]
     // forward
-    int splits;                    // slices of the vocabulary
     bool narrow;                   // tiles of 64 tokens, not 256
-    float *part;                   // [splits, rows_pad, 2]: maximum and sum of a row in a slice
-    float *row_loss;               // [rows_pad]
+    int stat_slots, stat_rounds;   // workgroups resident at once; rounds of them to consider
+    int stat_items;                // workgroups there are partial results for
+    float *part;                   // [token][slice] (maximum, sum)
+    float *row_loss;               // sum, mean: [N]
     float *loss;                   // scalar, or [N]
     // backward
     const float *g;                // gradient of loss
-    int g_stride;                  // none: elements between rows of g (0: one for all)
-    float *coef;                   // [rows_pad]: factor of a row of P
-    float *unscale;                // [1]: factor of the finished products
+    int g_stride;                  // none: elements between rows of g
+    float *coef;                   // none: [rows_pad] factor of a row of P; else null
+    float *unscale;                // none: [1] factor of the finished products
+    bool small;                    // tiles of 128, not 256
+    int slots;                     // workgroups resident at once
     int piece, pieces;             // vocabulary columns of a piece; pieces
     int v0, v1;                    // the piece whose dW and dx are formed, from P
     const void *P;                 // [rows_pad, piece]
     int p0, p1;                    // the piece whose P is formed, into Pn
     void *Pn;
-    int xcap;                      // dx: tiles of 256 tokens there are sums for, in all slices
-    float *acc;                    // [xcap * 256, d]
+    int strip;                     // tiles of P an item
+    int xcap;                      // dx: token tiles there are sums for, in all slices
+    float *acc;                    // [xcap tiles, dp]
     int wsplit;                    // dW: slices of the tokens
     float *wacc;                   // [wsplit, piece, dp]; only with slices
     void *dx, *dw;                 // [N, d], [V, d]; null: not wanted
 };
 
-hipError_t launch_xent_pack(const XentArgs &a, hipStream_t st);
 hipError_t launch_xent_fwd(const XentArgs &a, hipStream_t st);
 hipError_t launch_xent_pad_weight(const void *w, int64_t w_stride, void *out, int V, int d, int dp, int type, hipStream_t st);
 hipError_t launch_xent_bwd_prepare(const XentArgs &a, hipStream_t st);

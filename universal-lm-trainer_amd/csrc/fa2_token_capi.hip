@@ -67,8 +67,10 @@ int check_norm_types(int x, int res, int y, bool fp8) {
 // ---------------------------------------------------------------------------
 struct XentPlan {
     int rows_pad, dp;
-    bool narrow;
-    int splits, piece, pieces, xcap, wsplit;
+    bool narrow, small;
+    int stat_slots, stat_rounds, stat_items;
+    int slots, piece, pieces, strip, xcap;
+    int wsplit, wsplit_last;
     // offsets in the state
     size_t count, lse, tgt, rowmap, pos, xc, state_bytes;
     // offsets in the forward's workspace
@@ -77,25 +79,44 @@ struct XentPlan {
     size_t b_weight, coef, unscale, P[2], acc, wacc, bwd_bytes;
 };
 
+int64_t clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// Sizes that must not depend on how many tokens count, which only the device knows;
+// the kernels choose the slices of the forward and of dx within them.
 XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     using namespace fa2;
     XentPlan p;
     p.rows_pad = (int)((rows + XENT_PAD - 1) / XENT_PAD * XENT_PAD);
     p.dp = (d + XENT_KPAD - 1) / XENT_KPAD * XENT_KPAD;
-    const int64_t R = p.rows_pad, nd = (d + 255) / 256, tiles = (V + 255) / 256;
-    auto clamp = [](int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; };
+    const int64_t R = p.rows_pad;
+    // Forward.  Up to 1024 tokens in tiles of 64, three workgroups a compute unit; else of 256, one.
     p.narrow = R <= 1024;
-    p.splits = (int)clamp(256 / (p.narrow ? (rows + 63) / 64 : R / 256), 1, tiles);
-    // A piece's P is at most 256 MiB (twice, with more than one piece), in equal pieces.
-    const int64_t rt = R / 256, most = clamp(((int64_t)256 << 20) / (2 * R) / XENT_PAD * XENT_PAD, XENT_PAD, 1 << 24);
+    p.stat_slots = p.narrow ? 768 : 256;
+    p.stat_rounds = p.narrow ? 1 : 4;
+    const int64_t token_tiles = p.narrow ? (rows + 63) / 64 : R / 256;
+    p.stat_items = (int)(token_tiles > p.stat_slots * p.stat_rounds ? token_tiles : p.stat_slots * p.stat_rounds);
+    const int64_t v_tiles = (V + (p.narrow ? XENT_NARROW_V : 256) - 1) / (p.narrow ? XENT_NARROW_V : 256);
+    if (p.stat_items > token_tiles * v_tiles) p.stat_items = (int)(token_tiles * v_tiles);
+    // Backward.  A piece's P is at most 256 MiB (twice, with more than one piece), in equal pieces.
+    const int64_t most = clamp(((int64_t)256 << 20) / (2 * R) / XENT_PAD * XENT_PAD, XENT_PAD, 1 << 24);
     p.pieces = (int)((V + most - 1) / most);
     p.piece = (int)(((V + p.pieces - 1) / p.pieces + XENT_PAD - 1) / XENT_PAD * XENT_PAD);
     p.pieces = (V + p.piece - 1) / p.piece;
-    // dx: sums for all token tiles, or, when those are few, for slices up to one item a compute unit.
-    p.xcap = (int)(rt > 256 / nd ? rt : nd < 256 ? 256 / nd : 1);
-    // dW: its k, the tokens, in slices no longer than a compute unit's share of a launch (stages of 64 k).
-    const int64_t nv = p.piece / 256, share = nv * rt * (nd * 8 + (p.pieces > 1 ? p.dp / 64 + 4 : 0)) / 256;
-    p.wsplit = (int)clamp((4 * rt + share) / (share > 4 ? share + 1 : 4), 1, 16);
+    // Tiles of 128 where P has fewer tiles of 256 than there are compute units.
+    p.small = (R / 256) * (p.piece / 256) < 256;
+    p.slots = p.small ? 512 : 256;
+    const int64_t tt = p.small ? 128 : 256, rt = R / tt, nd = (d + tt - 1) / tt, nv = p.piece / tt;
+    p.strip = p.small ? 1 : (int)clamp(rt * nv / (4 * p.slots), 1, 4);
+    // dx: sums for all token tiles, or, when those are few, for slices up to one item a slot.
+    p.xcap = (int)(rt * nd > p.slots ? rt : clamp(p.slots / nd, 1, p.slots));
+    // dW: its k, the tokens, in slices no longer than a slot's share of a launch, and
+    // than a third of it in the last launch, which has no P to fill the slots with
+    // (stages of 64 k).
+    const int64_t kt = rt * (tt / 64), both = nv * rt * (nd * 2 * (tt / 64)) / p.slots, fill = nv * rt * (p.dp / 64 + 4) / p.slots;
+    auto slices = [&](int64_t len) { return (int)clamp((kt + len - 1) / (len > 4 ? len : 4), 1, p.pieces > 1 ? 4 : 16); };
+    p.wsplit = slices(both + fill);
+    p.wsplit_last = slices(both / 3);
+    const int wmax = p.wsplit > p.wsplit_last ? p.wsplit : p.wsplit_last;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += up256(bytes); return o; };
     p.count = take(256);
@@ -108,8 +129,8 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     const size_t wbytes = d % XENT_KPAD ? (size_t)V * p.dp * 2 : 0;
     at = 0;
     p.f_weight = take(wbytes);
-    p.part = take((size_t)p.splits * R * 8);
-    p.row_loss = take(R * 4);
+    p.part = take((size_t)p.stat_items * (p.narrow ? 64 : 256) * 8);
+    p.row_loss = take((size_t)rows * 4);
     p.fwd_bytes = at;
     at = 0;
     p.b_weight = take(wbytes);
@@ -117,8 +138,8 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     p.unscale = take(256);
     p.P[0] = take((size_t)R * p.piece * 2);
     p.P[1] = p.pieces > 1 ? take((size_t)R * p.piece * 2) : p.P[0];
-    p.acc = take((size_t)p.xcap * 256 * d * 4);
-    p.wacc = take(p.wsplit > 1 ? (size_t)p.wsplit * p.piece * p.dp * 4 : 0);
+    p.acc = take((size_t)p.xcap * tt * p.dp * 4);
+    p.wacc = take(wmax > 1 ? (size_t)wmax * p.piece * p.dp * 4 : 0);
     p.bwd_bytes = at;
     return p;
 }
@@ -178,12 +199,16 @@ fa2::XentArgs xent_args(const fa2_xent_params *p, const XentPlan &pl) {
     a.rowmap = reinterpret_cast<int *>(s + pl.rowmap);
     a.pos = reinterpret_cast<int *>(s + pl.pos);
     a.xc = s + pl.xc;
-    a.splits = pl.splits;
     a.narrow = pl.narrow;
+    a.stat_slots = pl.stat_slots;
+    a.stat_rounds = pl.stat_rounds;
+    a.stat_items = pl.stat_items;
+    a.small = pl.small;
+    a.slots = pl.slots;
     a.piece = pl.piece;
     a.pieces = pl.pieces;
+    a.strip = pl.strip;
     a.xcap = pl.xcap;
-    a.wsplit = pl.wsplit;
     return a;
 }
 
@@ -318,8 +343,8 @@ int fa2_xent_fwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
     a.part = reinterpret_cast<float *>(w + pl.part);
     a.row_loss = reinterpret_cast<float *>(w + pl.row_loss);
     a.loss = p->loss;
-    hipError_t e = fa2::launch_xent_pack(a, st);
-    if (e == hipSuccess && p->hidden % fa2::XENT_KPAD) {
+    hipError_t e = hipSuccess;
+    if (p->hidden % fa2::XENT_KPAD) {
         e = fa2::launch_xent_pad_weight(p->weight, p->weight_stride, w + pl.f_weight, a.V, a.d, a.dp, a.type, st);
         a.w = w + pl.f_weight;
         a.w_stride = a.dp;
@@ -345,8 +370,9 @@ int fa2_xent_bwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
     const hipStream_t st = (hipStream_t)stream;
     a.g = p->dloss;
     a.g_stride = (int)p->dloss_stride;
-    a.coef = reinterpret_cast<float *>(w + pl.coef);
-    a.unscale = reinterpret_cast<float *>(w + pl.unscale);
+    const bool per_row = p->reduction == FA2_REDUCE_NONE;
+    a.coef = per_row ? reinterpret_cast<float *>(w + pl.coef) : nullptr;
+    a.unscale = per_row ? reinterpret_cast<float *>(w + pl.unscale) : nullptr;
     a.acc = reinterpret_cast<float *>(w + pl.acc);
     a.wacc = reinterpret_cast<float *>(w + pl.wacc);
     a.dx = p->rows > 0 ? p->dx : nullptr;
@@ -357,7 +383,7 @@ int fa2_xent_bwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
         a.w = w + pl.b_weight;
         a.w_stride = a.dp;
     }
-    if (e == hipSuccess) e = fa2::launch_xent_bwd_prepare(a, st);
+    if (e == hipSuccess && per_row) e = fa2::launch_xent_bwd_prepare(a, st);
     for (int i = 0; i <= a.pieces && e == hipSuccess; ++i) {   // P of piece i beside the gradients of piece i - 1
         auto edge = [&](int k) { return (int64_t)k * a.piece < a.V ? k * a.piece : a.V; };
         a.v0 = i > 0 ? edge(i - 1) : 0;
@@ -366,6 +392,7 @@ int fa2_xent_bwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
         a.p1 = edge(i + 1);
         a.P = w + pl.P[(i + 1) & 1];
         a.Pn = w + pl.P[i & 1];
+        a.wsplit = i == a.pieces ? pl.wsplit_last : pl.wsplit;
         e = fa2::launch_xent_grad(a, st);
     }
     if (e == hipSuccess && a.dx) e = fa2::launch_xent_bwd_finish(a, st);

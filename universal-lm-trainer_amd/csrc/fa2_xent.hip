@@ -30,68 +30,106 @@ namespace {
 
 constexpr float P_SCALE = 32768.f;
 
+// Elements of XentArgs::count.
+enum { N_TOKENS = 0, STAT_SPLITS = 1 };
+
 // ---------------------------------------------------------------------------
 // Packing
 // ---------------------------------------------------------------------------
 
-// One workgroup: positions of the tokens that count, in order.
-__global__ __launch_bounds__(1024) void xent_scan_kernel(const XentArgs a) {
-    __shared__ int wave_sum[16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int before = 0;   // tokens that count in earlier rounds
-    for (int64_t r0 = 0; r0 < a.rows; r0 += 1024) {
-        const int64_t i = r0 + threadIdx.x;
-        const int64_t t = i < a.rows ? a.target[i] : a.ignore;
-        const bool in = i < a.rows && t != a.ignore;
-        const uint64_t m = __ballot(in);
-        if (lane == 0) wave_sum[wave] = __popcll(m);
-        __syncthreads();
-        int mine = before, all = before;
-#pragma unroll
-        for (int w = 0; w < 16; ++w) {
-            mine += w < wave ? wave_sum[w] : 0;
-            all += wave_sum[w];
+// Slices of the vocabulary for the forward: the workgroups (token tiles x slices)
+// fill the slots once, or a few times where that leaves fewer of them idle; the
+// cost of a choice is its rounds times the tiles of a slice.
+__device__ __forceinline__ int stat_splits(const XentArgs &a, int n) {
+    const int tm = a.narrow ? XENT_NARROW_V : 256, rt = max(1, (n + (a.narrow ? 64 : 256) - 1) / (a.narrow ? 64 : 256));
+    const int tiles = (a.V + tm - 1) / tm;
+    int best = 1, cost = INT32_MAX;
+    for (int k = 1; k <= a.stat_rounds; ++k) {
+        const int s = max(1, min(tiles, k * a.stat_slots / rt));
+        const int c = (rt * s + a.stat_slots - 1) / a.stat_slots * ((tiles + s - 1) / s);
+        if (c < cost) {
+            cost = c;
+            best = s;
         }
-        mine += __popcll(m & ((1ull << lane) - 1));
-        if (i < a.rows) a.pos[i] = in ? mine : -1;
-        if (in) {
-            a.rowmap[mine] = (int)i;
-            a.tgt[mine] = t >= 0 && t < a.V ? (int)t : -1;
-        }
-        before = all;
-        __syncthreads();
     }
-    if (threadIdx.x == 0) a.count[0] = before;
-    for (int j = before + threadIdx.x; j < a.rows_pad; j += 1024) {
-        a.rowmap[j] = -1;
-        a.tgt[j] = -1;
-    }
+    return best;
 }
 
-// Packed copy of the hidden states, one wave a row; zeros behind the last token
-// and the last column.
+// Every workgroup counts through all targets, and does its share of the rest: the
+// packed rows' token, target and states (zeros behind the last column and up to a
+// whole tile of rows), and the tokens' packed rows.
+constexpr int PACK_ROWS = 64;   // packed rows a workgroup has at a time
+
 template <typename T>
-__global__ __launch_bounds__(256) void xent_pack_kernel(const XentArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int j = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (j >= a.rows_pad) return;
-    const int r = a.rowmap[j];
-    T *o = static_cast<T *>(a.xc) + (int64_t)j * a.dp;
-    const T *x = static_cast<const T *>(a.x) + (int64_t)r * a.x_stride;
-    const bool vec = a.x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+__global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
+    __shared__ int wave_sum[16];
+    __shared__ int src[PACK_ROWS];
     typedef typename vec_of<T>::v8 v8;
-    for (int c = lane * 8; c < a.dp; c += 512) {
-        v8 v = {};
-        if (r >= 0) {
-            if (vec && c + 8 <= a.d) {
-                v = *reinterpret_cast<const v8 *>(x + c);
-            } else {
+    constexpr int Q = 16;   // targets a thread has at a time
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t i0 = a.rows * blockIdx.x / gridDim.x, i1 = a.rows * (blockIdx.x + 1) / gridDim.x;
+    const bool vec = a.x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.d % 8 == 0;
+    for (int j0 = blockIdx.x * PACK_ROWS; j0 < a.rows_pad; j0 += gridDim.x * PACK_ROWS) {
+        int n = 0;   // tokens that count so far
+        for (int64_t r0 = 0; r0 < a.rows; r0 += 1024 * Q) {
+            const int64_t first = r0 + wave * (64 * Q) + lane;
+            int64_t t[Q];
+            uint64_t m[Q];
+            int mine = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (c + e < a.d) v[e] = x[c + e];
+            for (int q = 0; q < Q; ++q) t[q] = first + q * 64 < a.rows ? a.target[first + q * 64] : a.ignore;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                m[q] = __ballot(first + q * 64 < a.rows && t[q] != a.ignore);
+                mine += __popcll(m[q]);
+            }
+            __syncthreads();   // the last round's sums have been read
+            if (lane == 0) wave_sum[wave] = mine;
+            __syncthreads();
+            int at = n;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+                at += w < wave ? wave_sum[w] : 0;
+                n += wave_sum[w];
+            }
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                const int64_t i = first + q * 64;
+                const bool in = m[q] >> lane & 1;
+                const int j = at + __popcll(m[q] & ((1ull << lane) - 1));
+                at += __popcll(m[q]);
+                if (i >= i0 && i < i1) a.pos[i] = in ? j : -1;
+                if (in && j >= j0 && j < j0 + PACK_ROWS) {
+                    src[j - j0] = (int)i;
+                    a.rowmap[j] = (int)i;
+                    a.tgt[j] = t[q] >= 0 && t[q] < a.V ? (int)t[q] : -1;
+                }
             }
         }
-        *reinterpret_cast<v8 *>(o + c) = v;
+        if (j0 == 0 && threadIdx.x == 0) {
+            a.count[N_TOKENS] = n;
+            a.count[STAT_SPLITS] = stat_splits(a, n);
+        }
+        if (threadIdx.x < PACK_ROWS && j0 + (int)threadIdx.x >= n) a.tgt[j0 + threadIdx.x] = -1;
+        __syncthreads();
+        // Pieces of 8 elements, a thread's next to those of its neighbours.
+        const int rows = min(PACK_ROWS, (n + XENT_PAD - 1) / XENT_PAD * XENT_PAD - j0), per = a.dp / 8;
+        for (int p = threadIdx.x; p < rows * per; p += 1024) {
+            const int r = p / per, c = (p - r * per) * 8;
+            v8 v = {};
+            if (j0 + r < n) {
+                const T *x = static_cast<const T *>(a.x) + (int64_t)src[r] * a.x_stride;
+                if (vec) {
+                    if (c < a.d) v = *reinterpret_cast<const v8 *>(x + c);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (c + e < a.d) v[e] = x[c + e];
+                }
+            }
+            *reinterpret_cast<v8 *>(static_cast<T *>(a.xc) + (int64_t)(j0 + r) * a.dp + c) = v;
+        }
+        __syncthreads();   // src is free
     }
 }
 
@@ -101,6 +139,13 @@ template <typename T>
 __global__ __launch_bounds__(256) void xent_pad_weight_kernel(const T *w, int64_t stride, T *out, int V, int d, int dp) {
     for (int64_t r = blockIdx.x; r < V; r += gridDim.x)
         for (int c = threadIdx.x; c < dp; c += 256) out[r * dp + c] = c < d ? w[r * stride + c] : (T)0.f;
+}
+
+// Workgroups go to the eight XCDs in turn: the l-th of n items, numbered so that an
+// XCD's items are neighbours (their operands meet in its L2).
+__device__ __forceinline__ int xcd_item(int l, int n) {
+    const int x = l & 7;
+    return x * (n >> 3) + min(x, n & 7) + (l >> 3);
 }
 
 // ---------------------------------------------------------------------------
@@ -114,23 +159,25 @@ __device__ __forceinline__ void join_max_sum(float &m, float &l, float m2, float
     m = n;
 }
 
-// Maximum and sum of exp of each packed row over a slice of the vocabulary.  The
-// M side are vocabulary rows, the N side tokens: a lane holds one token's logits.
-// Each lane keeps a reference r and the sum of exp(z - r) of the logits it has
-// seen.  r is the maximum of the lane's first tile and moves only when a sum
-// passes 2^100: fp32 holds the terms of any larger logits until then.  The slice's
-// tiles are one stream of stages: the next tile's transfers run behind the
-// exponentials.
-template <typename T, int NP, int WM, int WN>
+// Maximum and sum of exp of each packed row over a slice of the vocabulary.  The M
+// side are vocabulary rows, the N side tokens: a lane holds one token's logits.  Each
+// lane keeps a reference r and the sum of exp(z - r) of the logits it has seen.  r is
+// the maximum of the lane's first tile and moves only when a sum passes 2^100: fp32
+// holds the terms of any larger logits until then.  The slice's tiles are one stream
+// of stages: the next tile's transfers run behind the exponentials.
+template <typename T, int MP, int NP, int WM, int WN>
 __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
-    typedef Product<T, true, true, 4, NP, WM, WN> Pr;
+    typedef Product<T, true, true, false, MP, NP, WM, WN> Pr;
     constexpr int MI = Pr::MI, NI = Pr::NI;
     __shared__ __align__(16) char mem[Pr::LDS];
-    const int nr = a.rows_pad / Pr::TN;
-    const int rb = blockIdx.x % nr, split = blockIdx.x / nr;
-    if (rb * Pr::TN >= a.count[0]) return;
+    const int n = a.count[N_TOKENS], splits = a.count[STAT_SPLITS];
+    const int rt = (n + Pr::TN - 1) / Pr::TN;
+    if ((int)blockIdx.x >= rt * splits) return;
+    // groups of 8 token tiles, in a group the tokens fastest: a slice's weights meet in one XCD's L2
+    const int item = xcd_item(blockIdx.x, rt * splits), g = item / (8 * splits), gs = min(8, rt - 8 * g), in_g = item - g * 8 * splits;
+    const int rb = 8 * g + in_g % gs, split = in_g / gs;
     const int tiles = (a.V + Pr::TM - 1) / Pr::TM;
-    const int t0 = (int)((int64_t)tiles * split / a.splits), t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
+    const int t0 = (int)((int64_t)tiles * split / splits), t1 = (int)((int64_t)tiles * (split + 1) / splits);
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
     Pr pr;
     pr.init(mem);
@@ -217,69 +264,60 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
         float m = jm[i], l = jl[i];
 #pragma unroll
         for (int w = 1; w < WM; ++w) join_max_sum(m, l, jm[w * Pr::TN + i], jl[w * Pr::TN + i]);
-        *(reinterpret_cast<f2 *>(a.part) + (int64_t)split * a.rows_pad + rb * Pr::TN + i) = f2{m, l};
+        reinterpret_cast<f2 *>(a.part)[(int64_t)(rb * Pr::TN + i) * splits + split] = f2{m, l};
     }
 }
 
-// One wave a packed row: joins the slices, and the target's logit as a product of
-// its own.
+// One wave a token: joins its slices, and forms the target's logit as a product of its
+// own (found among the tiles' logits it cost the forward's kernel 6%).
 template <typename T>
 __global__ __launch_bounds__(256) void xent_join_kernel(const XentArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int j = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (j >= a.count[0]) return;
-    float m = -INFINITY, l = 0.f;
-    for (int s = lane; s < a.splits; s += 64) {
-        const f2 p = *(reinterpret_cast<const f2 *>(a.part) + (int64_t)s * a.rows_pad + j);
-        join_max_sum(m, l, p[0], p[1]);
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) join_max_sum(m, l, __shfl_xor(m, o), __shfl_xor(l, o));
-    const float lse = m + __logf(l);
-    const int t = a.tgt[j];
-    float z = 0.f;
-    if (t >= 0) {
-        const T *x = static_cast<const T *>(a.xc) + (int64_t)j * a.dp;
-        const T *w = static_cast<const T *>(a.w) + (int64_t)t * a.w_stride;
+    const int lane = threadIdx.x & 63, splits = a.count[STAT_SPLITS];
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= a.rows) return;
+    const int j = a.pos[i];
+    float loss = 0.f;
+    if (j >= 0) {
+        const int t = a.tgt[j];
         typedef typename vec_of<T>::v8 v8;
+        const T *x = static_cast<const T *>(a.xc) + (int64_t)j * a.dp;
+        const T *w = static_cast<const T *>(a.w) + (int64_t)max(t, 0) * a.w_stride;
+        float z = 0.f;
         for (int c = lane * 8; c < a.dp; c += 512) {
             const f8 xv = __builtin_convertvector(*reinterpret_cast<const v8 *>(x + c), f8);
             const f8 wv = __builtin_convertvector(*reinterpret_cast<const v8 *>(w + c), f8);
 #pragma unroll
             for (int e = 0; e < 8; ++e) z += xv[e] * wv[e];
         }
+        float m = -INFINITY, l = 0.f;
+        for (int s = lane; s < splits; s += 64) {
+            const f2 p = reinterpret_cast<const f2 *>(a.part)[(int64_t)j * splits + s];
+            join_max_sum(m, l, p[0], p[1]);
+        }
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) z += __shfl_xor(z, o);
+        for (int o = 32; o >= 1; o >>= 1) {
+            join_max_sum(m, l, __shfl_xor(m, o), __shfl_xor(l, o));
+            z += __shfl_xor(z, o);
+        }
+        const float lse = m + logf(l);
+        loss = t >= 0 ? lse - z : NAN;   // a target outside the vocabulary
+        if (lane == 0) a.lse[j] = lse;
     }
-    if (lane == 0) {
-        const float loss = t >= 0 ? lse - z : NAN;   // a target outside the vocabulary
-        a.lse[j] = lse;
-        if (a.reduction == FA2_REDUCE_NONE)
-            a.loss[a.rowmap[j]] = loss;
-        else
-            a.row_loss[j] = loss;
-    }
+    if (lane == 0) (a.reduction == FA2_REDUCE_NONE ? a.loss : a.row_loss)[i] = loss;
 }
 
-// none: zeros for the tokens that do not count.
-__global__ __launch_bounds__(256) void xent_ignored_kernel(const XentArgs a) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.rows; i += (int64_t)gridDim.x * 256)
-        if (a.pos[i] < 0) a.loss[i] = 0.f;
-}
-
-// sum, mean: one workgroup adds the rows' losses in a fixed order.
+// sum, mean: one workgroup adds the tokens' losses in a fixed order.
 __global__ __launch_bounds__(1024) void xent_sum_kernel(const XentArgs a) {
-    __shared__ double s[16];
-    const int n = a.count[0];
+    __shared__ double sums[16];
     double v = 0.;
-    for (int j = threadIdx.x; j < n; j += 1024) v += a.row_loss[j];
+    for (int64_t i = threadIdx.x; i < a.rows; i += 1024) v += a.row_loss[i];
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < 16; ++i) v += s[i];
-        a.loss[0] = (float)(a.reduction == FA2_REDUCE_MEAN ? v / n : v);   // mean of none: 0 / 0, as torch
+        for (int k = 1; k < 16; ++k) v += sums[k];
+        a.loss[0] = (float)(a.reduction == FA2_REDUCE_MEAN ? v / a.count[N_TOKENS] : v);   // mean of none: 0 / 0, as torch
     }
 }
 
@@ -287,89 +325,72 @@ __global__ __launch_bounds__(1024) void xent_sum_kernel(const XentArgs a) {
 // Backward
 // ---------------------------------------------------------------------------
 
-// Factors of the rows of P, and the factor of the finished products.  sum and
-// mean: every row has P_SCALE; none: the row's gradient over the largest one.
+// none: each row of P is scaled by its gradient over the largest one, which the
+// finished products are multiplied with.  (sum and mean: every row has 1.)
 __global__ __launch_bounds__(1024) void xent_coef_kernel(const XentArgs a) {
     __shared__ float s[16];
-    const int n = a.count[0];
+    const int n = a.count[N_TOKENS];
     float top = 0.f;
-    if (a.reduction == FA2_REDUCE_NONE) {
-        for (int j = threadIdx.x; j < n; j += 1024) {
-            const float v = fabsf(a.g[(int64_t)a.rowmap[j] * a.g_stride]);
-            top = (v > top || v != v) ? v : top;
-        }
+    auto larger = [](float a, float b) FA2_INLINE { return (b > a || b != b) ? b : a; };
+    for (int j = threadIdx.x; j < n; j += 1024) top = larger(top, fabsf(a.g[(int64_t)a.rowmap[j] * a.g_stride]));
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            const float v = __shfl_xor(top, o);
-            top = (v > top || v != v) ? v : top;
-        }
-        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
-        __syncthreads();
-        top = 0.f;
-        for (int i = 0; i < 16; ++i) top = (s[i] > top || s[i] != s[i]) ? s[i] : top;
+    for (int o = 32; o >= 1; o >>= 1) top = larger(top, __shfl_xor(top, o));
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = 0.f;
+    for (int i = 0; i < 16; ++i) top = larger(top, s[i]);
+    for (int j = threadIdx.x; j < n; j += 1024) {
+        const float v = a.g[(int64_t)a.rowmap[j] * a.g_stride];
+        a.coef[j] = v == 0.f ? 0.f : v / top;
     }
-    for (int j = threadIdx.x; j < a.rows_pad; j += 1024) {
-        float f = 0.f;
-        if (j < n) {
-            f = P_SCALE;
-            if (a.reduction == FA2_REDUCE_NONE) {
-                const float v = a.g[(int64_t)a.rowmap[j] * a.g_stride];
-                f = v == 0.f ? 0.f : v / top * P_SCALE;
-            }
-            if (a.tgt[j] < 0) f = NAN;
-        }
-        a.coef[j] = f;
-    }
-    if (threadIdx.x == 0) {
-        const float u = a.reduction == FA2_REDUCE_NONE ? top : a.reduction == FA2_REDUCE_MEAN ? a.g[0] / (float)n : a.g[0];
-        a.unscale[0] = n ? u / P_SCALE : 0.f;
-    }
+    if (threadIdx.x == 0) a.unscale[0] = top / P_SCALE;
+}
+
+// What the products of P are multiplied with.
+__device__ __forceinline__ float xent_unscale(const XentArgs &a, int n) {
+    if (n == 0) return 0.f;
+    if (a.reduction == FA2_REDUCE_NONE) return a.unscale[0];
+    return (a.reduction == FA2_REDUCE_MEAN ? a.g[0] / (float)n : a.g[0]) / P_SCALE;
 }
 
 // The work of one launch of the backward: dW and dx of a piece, and P of the piece
 // after it, as items of one grid, the long ones first; P's many short items fill the
-// compute units that the others leave.  Lengths are in stages of 64 k.
+// compute units that the others leave.  Lengths are in stages of 64 k; tiles are
+// 64 MP on a side.
 struct XentWork {
-    int rt;            // tiles of 256 tokens that count
+    int rt;            // tiles of tokens that count
     int dw, dx, p;     // items
     int xs;            // slices of dx's k
 };
 
-constexpr int P_STRIP = 4;       // tiles of P an item
 constexpr int P_TILE_EXTRA = 4;  // stages that the softmax of a tile of P takes as long as
 
+template <int MP>
 __device__ __forceinline__ XentWork xent_work(const XentArgs &a, int n) {
+    constexpr int TT = 64 * MP;
     XentWork k;
-    const int nd = (a.d + 255) / 256, nv = (a.v1 - a.v0 + 255) / 256, nvp = (a.p1 - a.p0 + 255) / 256;
-    k.rt = (n + 255) / 256;
-    // Slices of dx: no longer than three quarters of a compute unit's share of a
-    // launch (with pieces of full width; the same number for every piece).
-    const int64_t full = a.piece / 256;
-    const int64_t total = full * k.rt * (nd * 8 + (a.pieces > 1 ? a.dp / PK + P_TILE_EXTRA : 0));
-    const int share = (int)max((int64_t)4, total * 3 / (4 * 256));
+    const int nd = (a.d + TT - 1) / TT, nv = (a.v1 - a.v0 + TT - 1) / TT, nvp = (a.p1 - a.p0 + TT - 1) / TT;
+    k.rt = (n + TT - 1) / TT;
+    // Slices of dx: no longer than three quarters of a slot's share of a launch (with
+    // pieces of full width; the same number for every piece).
+    const int64_t total = (int64_t)(a.piece / TT) * k.rt * (nd * 2 * MP + (a.pieces > 1 ? a.dp / PK + P_TILE_EXTRA : 0));
+    const int share = (int)max((int64_t)4, total * 3 / (4 * a.slots));
     k.xs = max(1, min((a.piece / PK + share - 1) / share, a.xcap / max(k.rt, 1)));
     k.dw = a.dw ? nd * nv * a.wsplit : 0;
     k.dx = a.dx && nv > 0 ? nd * k.rt * k.xs : 0;
-    k.p = k.rt * ((nvp + P_STRIP - 1) / P_STRIP);
+    k.p = k.rt * ((nvp + a.strip - 1) / a.strip);
     return k;
 }
 
-// Workgroups go to the eight XCDs in turn: the l-th of n items, numbered so that an
-// XCD's items are neighbours (their operands meet in its L2).
-__device__ __forceinline__ int xcd_item(int l, int n) {
-    const int x = l & 7;
-    return x * (n >> 3) + min(x, n & 7) + (l >> 3);
-}
-
-// P_STRIP tiles of P: logits again, softmax, minus one at the target, times the row's
-// factor; M side vocabulary rows, N side tokens.
-template <typename T>
+// a.strip tiles of P: logits again, softmax, minus one at the target; M side
+// vocabulary rows, N side tokens.  In units of 1 / P_SCALE, times the row's factor.
+template <typename T, int MP>
 __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k, int item, int n, char *mem, char *out) {
-    typedef Product<T, true, true, 4, 4, 2, 4> Pr;
-    const int tiles = (a.p1 - a.p0 + 255) / 256, strips = (tiles + P_STRIP - 1) / P_STRIP;
+    typedef Product<T, true, true, false, MP, MP, 2, 4> Pr;
+    const int tiles = (a.p1 - a.p0 + Pr::TM - 1) / Pr::TM, strips = (tiles + a.strip - 1) / a.strip;
     // groups of 8 token tiles, in a group the tokens fastest
     const int g = item / (8 * strips), gs = min(8, k.rt - 8 * g), in = item - g * 8 * strips;
-    const int rb = 8 * g + in % gs, t0 = in / gs * P_STRIP, t1 = min(tiles, t0 + P_STRIP);
+    const int rb = 8 * g + in % gs, t0 = in / gs * a.strip, t1 = min(tiles, t0 + a.strip);
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
     Pr pr;
     pr.init(mem);
@@ -380,9 +401,10 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
 #pragma unroll
     for (int j = 0; j < Pr::NI; ++j) {
         const int row = rb * Pr::TN + pr.wn + 32 * j + c;
-        f[j] = a.coef[row];
-        sub[j] = row < n ? a.lse[row] * LOG2E : 0.f;
-        tgt[j] = a.tgt[row] - pr.wm;
+        const int t = a.tgt[row];
+        f[j] = row >= n ? 0.f : t < 0 ? NAN : a.coef ? a.coef[row] : 1.f;
+        sub[j] = row < n ? a.lse[row] * LOG2E - 15.f : 0.f;   // P_SCALE = 2^15
+        tgt[j] = t - pr.wm;
     }
     int nt = t0, nk = 0;
     auto next = [&](int buf) FA2_INLINE {
@@ -409,16 +431,13 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(acc[i + h][j][r] * LOG2E - sub[j]) * f[j];
-                        acc[i + h][j][r] = f[j] != 0.f ? p : 0.f;
-                    }
+                    for (int r = 0; r < 16; ++r) acc[i + h][j][r] = __builtin_amdgcn_exp2f(acc[i + h][j][r] * LOG2E - sub[j]);
                     const int at = tgt[j] - v0 - 32 * (i + h);
                     if (__any(at >= 0 && at < 32)) {
                         FA2_COLD_BRANCH();
 #pragma unroll
                         for (int r = 0; r < 16; ++r)
-                            if (at == acc_row(r, g2)) acc[i + h][j][r] -= f[j];
+                            if (at == acc_row(r, g2)) acc[i + h][j][r] -= P_SCALE;
                     }
                     if (v0 + pr.wm + 32 * (i + h) + 32 > a.V) {   // rows past the vocabulary
                         FA2_COLD_BRANCH();
@@ -427,7 +446,7 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
                             if (v0 + pr.wm + 32 * (i + h) + acc_row(r, g2) >= a.V) acc[i + h][j][r] = 0.f;
                     }
                 }
-                store_rows<T>(acc[i][j], acc[i + 1][j], 1.f, blk, o + 32 * i, a.piece, 32, 64, true);
+                store_rows<T>(acc[i][j], acc[i + 1][j], f[j], blk, o + 32 * i, a.piece, 32, 64, true);
             }
         }
     }
@@ -435,12 +454,12 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
 
 // A tile of the piece's dW, or of a slice of its k: M side hidden columns, N side
 // vocabulary rows, K packed tokens.
-template <typename T>
+template <typename T, int MP>
 __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n, char *mem) {
-    typedef Product<T, false, false, 4, 4, 2, 4> Pr;
-    const int nd = (a.d + 255) / 256, nv = (a.v1 - a.v0 + 255) / 256;
+    typedef Product<T, false, false, true, MP, MP, 2, 4> Pr;
+    const int nd = (a.d + Pr::TM - 1) / Pr::TM, nv = (a.v1 - a.v0 + Pr::TM - 1) / Pr::TM;
     const int db = item % nd, vb = item / nd % nv, s = item / nd / nv;
-    const int kt = (n + 255) / 256 * (256 / PK);
+    const int kt = (n + Pr::TM - 1) / Pr::TM * MP;
     const int k0 = (int)((int64_t)kt * s / a.wsplit) * PK, k1 = (int)((int64_t)kt * (s + 1) / a.wsplit) * PK;
     Pr pr;
     pr.init(mem);
@@ -449,7 +468,7 @@ __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n,
     f16x acc[Pr::MI][Pr::NI];
     pr.run(k0, k1, acc);
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
-    const float u = a.unscale[0];
+    const float u = xent_unscale(a, n);
     char *blk = mem + (threadIdx.x >> 6) * 4096;
 #pragma unroll
     for (int j = 0; j < Pr::NI; ++j) {
@@ -479,10 +498,10 @@ __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n,
 
 // A tile of the piece's share of dx, or of a slice of its k: M side packed tokens, N
 // side hidden columns, K the piece.
-template <typename T>
+template <typename T, int MP>
 __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &k, int item, char *mem) {
-    typedef Product<T, true, false, 4, 4, 2, 4> Pr;
-    const int nd = (a.d + 255) / 256;
+    typedef Product<T, true, false, true, MP, MP, 2, 4> Pr;
+    const int nd = (a.d + Pr::TN - 1) / Pr::TN;
     const int db = item % nd, rb = item / nd % k.rt, s = item / nd / k.rt;
     const int kt = (a.v1 - a.v0 + PK - 1) / PK;
     const int k0 = (int)((int64_t)kt * s / k.xs) * PK, k1 = (int)((int64_t)kt * (s + 1) / k.xs) * PK;
@@ -496,64 +515,81 @@ __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &
 #pragma unroll
     for (int j = 0; j < Pr::NI; ++j) {
         const int col = db * Pr::TN + pr.wn + 32 * j + c;
-        if (col >= a.d) continue;
+        if (col >= a.dp) continue;
 #pragma unroll
         for (int i = 0; i < Pr::MI; ++i) {
-            float *o = a.acc + ((int64_t)(s * k.rt + rb) * Pr::TM + pr.wm + 32 * i) * a.d + col;
+            float *o = a.acc + ((int64_t)(s * k.rt + rb) * Pr::TM + pr.wm + 32 * i) * a.dp + col;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float *q = o + (int64_t)acc_row(r, g2) * a.d;
+                float *q = o + (int64_t)acc_row(r, g2) * a.dp;
                 *q = a.v0 == 0 ? acc[i][j][r] : *q + acc[i][j][r];
             }
         }
     }
 }
 
-template <typename T>
+// MP = 4: 160 KB of LDS, one workgroup a compute unit; P's output goes through LDS of
+// its own while the next tile's stages land.  MP = 2: 64 KB, two a unit, one tile of P
+// an item, whose output goes through the panels.
+template <typename T, int MP>
 __global__ __launch_bounds__(512, 2) void xent_grad_kernel(const XentArgs a) {
-    constexpr int PANELS = Product<T, true, true, 4, 4, 2, 4>::LDS;
-    __shared__ __align__(16) char mem[PANELS + 8 * 4096];
-    const int n = a.count[0];
-    const XentWork k = xent_work(a, n);
+    constexpr int PANELS = Product<T, true, true, false, MP, MP, 2, 4>::LDS;
+    __shared__ __align__(16) char mem[PANELS + (MP == 4 ? 8 * 4096 : 0)];
+    const int n = a.count[N_TOKENS];
+    const XentWork k = xent_work<MP>(a, n);
     int l = blockIdx.x;
-    const bool dw_first = (int64_t)k.rt * 4 * k.xs * PK > (int64_t)(a.v1 - a.v0) * a.wsplit;   // the longer ones
-    if (dw_first && l < k.dw) return xent_dw_item<T>(a, xcd_item(l, k.dw), n, mem);
+    const bool dw_first = (int64_t)n * k.xs > (int64_t)(a.v1 - a.v0) * a.wsplit;   // the longer ones
+    if (dw_first && l < k.dw) return xent_dw_item<T, MP>(a, xcd_item(l, k.dw), n, mem);
     l -= dw_first ? k.dw : 0;
-    if (l < k.dx) return xent_dx_item<T>(a, k, xcd_item(l, k.dx), mem);
+    if (l < k.dx) return xent_dx_item<T, MP>(a, k, xcd_item(l, k.dx), mem);
     l -= k.dx;
-    if (!dw_first && l < k.dw) return xent_dw_item<T>(a, xcd_item(l, k.dw), n, mem);
+    if (!dw_first && l < k.dw) return xent_dw_item<T, MP>(a, xcd_item(l, k.dw), n, mem);
     l -= dw_first ? 0 : k.dw;
-    if (l < k.p) xent_p_item<T>(a, k, xcd_item(l, k.p), n, mem, mem + PANELS);
+    if (l < k.p) xent_p_item<T, MP>(a, k, xcd_item(l, k.p), n, mem, mem + (MP == 4 ? PANELS : 0));
 }
 
-// dW of a piece whose k was sliced: the slices' sums in order.
+// Eight elements of a row of `cols`, rounded; whole 16-byte stores where `vec`.
 template <typename T>
-__global__ __launch_bounds__(256) void xent_dw_join_kernel(const XentArgs a) {
-    const float u = a.unscale[0];
-    const int64_t total = (int64_t)(a.v1 - a.v0) * a.d;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        const int64_t v = e / a.d;
-        const int c = (int)(e - v * a.d);
-        float x = 0.f;
-        for (int s = 0; s < a.wsplit; ++s) x += a.wacc[((int64_t)s * a.piece + v) * a.dp + c];
-        static_cast<T *>(a.dw)[(int64_t)a.v0 * a.d + e] = (T)(x * u);
+__device__ __forceinline__ void store8(T *row, int c, int cols, bool vec, const f8 &x) {
+    const typename vec_of<T>::v8 v = __builtin_convertvector(x, typename vec_of<T>::v8);
+    if (vec) {
+        *reinterpret_cast<typename vec_of<T>::v8 *>(row + c) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c + e < cols) row[c + e] = v[e];
     }
 }
 
-// dx of every token: the slices' sums, rounded once; zeros where a token does not count.
+// dW of a piece whose k was sliced: the slices' sums in order, one wave a row.
 template <typename T>
-__global__ __launch_bounds__(256) void xent_dx_out_kernel(const XentArgs a) {
-    const int64_t total = a.rows * a.d;
-    const XentWork k = xent_work(a, a.count[0]);
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        const int64_t i = e / a.d;
-        const int c = (int)(e - i * a.d), j = a.pos[i];
-        float v = 0.f;
-        if (j >= 0) {
-            for (int s = 0; s < k.xs; ++s) v += a.acc[((int64_t)s * k.rt * 256 + j) * a.d + c];
-            v *= a.unscale[0];
+__global__ __launch_bounds__(256) void xent_dw_join_kernel(const XentArgs a) {
+    const float u = xent_unscale(a, a.count[N_TOKENS]);
+    const int lane = threadIdx.x & 63;
+    for (int v = blockIdx.x * 4 + (threadIdx.x >> 6); v < a.v1 - a.v0; v += gridDim.x * 4)
+        for (int c = lane * 8; c < a.d; c += 512) {
+            f8 x = {};
+            for (int s = 0; s < a.wsplit; ++s) x += *reinterpret_cast<const f8 *>(a.wacc + ((int64_t)s * a.piece + v) * a.dp + c);
+            store8<T>(static_cast<T *>(a.dw) + (int64_t)(a.v0 + v) * a.d, c, a.d, a.d % 8 == 0, x * u);
         }
-        static_cast<T *>(a.dx)[e] = (T)v;
+}
+
+// dx of every token: the slices' sums, rounded once; zeros where a token does not
+// count.  One wave a token.
+template <typename T, int MP>
+__global__ __launch_bounds__(256) void xent_dx_out_kernel(const XentArgs a) {
+    const int n = a.count[N_TOKENS], lane = threadIdx.x & 63;
+    const XentWork k = xent_work<MP>(a, n);
+    const float u = xent_unscale(a, n);
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.rows; i += (int64_t)gridDim.x * 4) {
+        const int j = a.pos[i];
+        for (int c = lane * 8; c < a.d; c += 512) {
+            f8 x = {};
+            if (j >= 0)
+                for (int s = 0; s < k.xs; ++s)
+                    x += *reinterpret_cast<const f8 *>(a.acc + ((int64_t)s * k.rt * (64 * MP) + j) * a.dp + c);
+            store8<T>(static_cast<T *>(a.dx) + i * a.d, c, a.d, a.d % 8 == 0, x * u);
+        }
     }
 }
 
@@ -564,42 +600,33 @@ __global__ __launch_bounds__(256) void xent_dx_out_kernel(const XentArgs a) {
         if (e != hipSuccess) return e;                                     \
     } while (0)
 
+unsigned at_most(int64_t want, int64_t most) { return (unsigned)(want < most ? want : most); }
+
 template <typename T>
 hipError_t fwd(const XentArgs &a, hipStream_t st) {
+    FA2_LAUNCH(xent_pack_kernel<T>, at_most(a.rows_pad / PACK_ROWS, 1024), 1024);
     if (a.narrow)
-        FA2_LAUNCH((xent_stats_kernel<T, 1, 8, 1>), a.rows_pad / 64 * a.splits, 512);
+        FA2_LAUNCH((xent_stats_kernel<T, XENT_NARROW_V / 64, 1, XENT_NARROW_V / 32, 256 / XENT_NARROW_V>), a.stat_items, 512);
     else
-        FA2_LAUNCH((xent_stats_kernel<T, 4, 2, 4>), a.rows_pad / 256 * a.splits, 512);
-    if (a.reduction == FA2_REDUCE_NONE && a.rows > 0)
-        FA2_LAUNCH(xent_ignored_kernel, (unsigned)((a.rows + 255) / 256 < 4096 ? (a.rows + 255) / 256 : 4096), 256);
-    FA2_LAUNCH(xent_join_kernel<T>, a.rows_pad / 4, 256);
+        FA2_LAUNCH((xent_stats_kernel<T, 4, 4, 2, 4>), a.stat_items, 512);
+    if (a.rows > 0) FA2_LAUNCH(xent_join_kernel<T>, (unsigned)((a.rows + 3) / 4), 256);
     if (a.reduction != FA2_REDUCE_NONE) FA2_LAUNCH(xent_sum_kernel, 1, 1024);
     return hipSuccess;
 }
 
 // P of [p0, p1) beside dW and dx of [v0, v1); either may be empty.
-template <typename T>
+template <typename T, int MP>
 hipError_t grad(const XentArgs &a, hipStream_t st) {
-    const int rt = a.rows_pad / 256, nd = (a.d + 255) / 256, nv = (a.v1 - a.v0 + 255) / 256, np = (a.p1 - a.p0 + 255) / 256;
-    const int items = nd * nv * a.wsplit + (nv ? nd * a.xcap : 0) + rt * ((np + P_STRIP - 1) / P_STRIP);   // the most there can be
-    FA2_LAUNCH(xent_grad_kernel<T>, items, 512);
-    if (nv && a.dw && a.wsplit > 1) {
-        const int64_t want = ((int64_t)(a.v1 - a.v0) * a.d + 255) / 256;
-        FA2_LAUNCH(xent_dw_join_kernel<T>, (unsigned)(want < 8192 ? want : 8192), 256);
-    }
+    constexpr int TT = 64 * MP;
+    const int rt = a.rows_pad / TT, nd = (a.d + TT - 1) / TT, nv = (a.v1 - a.v0 + TT - 1) / TT, np = (a.p1 - a.p0 + TT - 1) / TT;
+    // the most items there can be
+    const int items = (a.dw ? nd * nv * a.wsplit : 0) + (a.dx && nv ? nd * a.xcap : 0) + rt * ((np + a.strip - 1) / a.strip);
+    if (items > 0) FA2_LAUNCH((xent_grad_kernel<T, MP>), items, 512);
+    if (nv && a.dw && a.wsplit > 1) FA2_LAUNCH(xent_dw_join_kernel<T>, at_most((a.v1 - a.v0 + 3) / 4, 8192), 256);
     return hipSuccess;
 }
 
 }  // namespace
-
-hipError_t launch_xent_pack(const XentArgs &a, hipStream_t st) {
-    FA2_LAUNCH(xent_scan_kernel, 1, 1024);
-    if (a.type == FA2_F16)
-        FA2_LAUNCH(xent_pack_kernel<_Float16>, a.rows_pad / 4, 256);
-    else
-        FA2_LAUNCH(xent_pack_kernel<__bf16>, a.rows_pad / 4, 256);
-    return hipSuccess;
-}
 
 hipError_t launch_xent_pad_weight(const void *w, int64_t w_stride, void *out, int V, int d, int dp, int type, hipStream_t st) {
     const dim3 grid(V < 4096 ? V : 4096), block(256);
@@ -622,16 +649,23 @@ hipError_t launch_xent_bwd_prepare(const XentArgs &a, hipStream_t st) {
 }
 
 hipError_t launch_xent_grad(const XentArgs &a, hipStream_t st) {
-    return a.type == FA2_F16 ? grad<_Float16>(a, st) : grad<__bf16>(a, st);
+    if (a.small) return a.type == FA2_F16 ? grad<_Float16, 2>(a, st) : grad<__bf16, 2>(a, st);
+    return a.type == FA2_F16 ? grad<_Float16, 4>(a, st) : grad<__bf16, 4>(a, st);
 }
 
 hipError_t launch_xent_bwd_finish(const XentArgs &a, hipStream_t st) {
-    const int64_t want = (a.rows * a.d + 255) / 256;
-    const unsigned grid = (unsigned)(want < 8192 ? want : 8192);
-    if (a.type == FA2_F16)
-        FA2_LAUNCH(xent_dx_out_kernel<_Float16>, grid, 256);
-    else
-        FA2_LAUNCH(xent_dx_out_kernel<__bf16>, grid, 256);
+    const unsigned grid = at_most((a.rows + 3) / 4, 8192);
+    if (a.type == FA2_F16) {
+        if (a.small)
+            FA2_LAUNCH((xent_dx_out_kernel<_Float16, 2>), grid, 256);
+        else
+            FA2_LAUNCH((xent_dx_out_kernel<_Float16, 4>), grid, 256);
+    } else {
+        if (a.small)
+            FA2_LAUNCH((xent_dx_out_kernel<__bf16, 2>), grid, 256);
+        else
+            FA2_LAUNCH((xent_dx_out_kernel<__bf16, 4>), grid, 256);
+    }
     return hipSuccess;
 }
 
