@@ -139,7 +139,7 @@ def test_module_surface():
     for name in ("rms_norm", "add_rms_norm", "rms_norm_fp8", "dropout", "linear_cross_entropy"):
         assert callable(getattr(fa, name))
     ext = fa.extension()
-    for op in ("rms_norm_fwd", "rms_norm_bwd", "rms_norm_fp8", "dropout", "xent_fwd", "xent_bwd"):
+    for op in ("rms_norm", "add_rms_norm", "rms_norm_fp8", "dropout", "linear_cross_entropy"):
         assert hasattr(ext, op)
 
 

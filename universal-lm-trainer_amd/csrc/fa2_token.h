@@ -103,6 +103,7 @@ struct XentArgs {
     float *lse;                    // [rows_pad]
     void *xc;                      // [rows_pad, dp]
     // forward
+    int pack_rows;                 // packed rows a workgroup has at a time
     bool narrow;                   // tiles of 64 tokens, not 256
     int stat_slots, stat_rounds;   // workgroups resident at once; rounds of them to consider
     int stat_items;                // workgroups there are partial results for

@@ -199,6 +199,7 @@ fa2::XentArgs xent_args(const fa2_xent_params *p, const XentPlan &pl) {
     a.rowmap = reinterpret_cast<int *>(s + pl.rowmap);
     a.pos = reinterpret_cast<int *>(s + pl.pos);
     a.xc = s + pl.xc;
+    a.pack_rows = pl.rows_pad <= 4096 ? 16 : 64;
     a.narrow = pl.narrow;
     a.stat_slots = pl.stat_slots;
     a.stat_rounds = pl.stat_rounds;

@@ -55,11 +55,11 @@ __device__ __forceinline__ int stat_splits(const XentArgs &a, int n) {
     return best;
 }
 
+constexpr int PACK_ROWS = 64;   // packed rows a workgroup has at a time, at most
+
 // Every workgroup counts through all targets, and does its share of the rest: the
 // packed rows' token, target and states (zeros behind the last column and up to a
 // whole tile of rows), and the tokens' packed rows.
-constexpr int PACK_ROWS = 64;   // packed rows a workgroup has at a time
-
 template <typename T>
 __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
     __shared__ int wave_sum[16];
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t i0 = a.rows * blockIdx.x / gridDim.x, i1 = a.rows * (blockIdx.x + 1) / gridDim.x;
     const bool vec = a.x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.d % 8 == 0;
-    for (int j0 = blockIdx.x * PACK_ROWS; j0 < a.rows_pad; j0 += gridDim.x * PACK_ROWS) {
+    for (int j0 = blockIdx.x * a.pack_rows; j0 < a.rows_pad; j0 += gridDim.x * a.pack_rows) {
         int n = 0;   // tokens that count so far
         for (int64_t r0 = 0; r0 < a.rows; r0 += 1024 * Q) {
             const int64_t first = r0 + wave * (64 * Q) + lane;
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
                 const int j = at + __popcll(m[q] & ((1ull << lane) - 1));
                 at += __popcll(m[q]);
                 if (i >= i0 && i < i1) a.pos[i] = in ? j : -1;
-                if (in && j >= j0 && j < j0 + PACK_ROWS) {
+                if (in && j >= j0 && j < j0 + a.pack_rows) {
                     src[j - j0] = (int)i;
                     a.rowmap[j] = (int)i;
                     a.tgt[j] = t[q] >= 0 && t[q] < a.V ? (int)t[q] : -1;
@@ -110,10 +110,10 @@ __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
             a.count[N_TOKENS] = n;
             a.count[STAT_SPLITS] = stat_splits(a, n);
         }
-        if (threadIdx.x < PACK_ROWS && j0 + (int)threadIdx.x >= n) a.tgt[j0 + threadIdx.x] = -1;
+        if ((int)threadIdx.x < a.pack_rows && j0 + (int)threadIdx.x >= n) a.tgt[j0 + threadIdx.x] = -1;
         __syncthreads();
         // Pieces of 8 elements, a thread's next to those of its neighbours.
-        const int rows = min(PACK_ROWS, (n + XENT_PAD - 1) / XENT_PAD * XENT_PAD - j0), per = a.dp / 8;
+        const int rows = min(a.pack_rows, (n + XENT_PAD - 1) / XENT_PAD * XENT_PAD - j0), per = a.dp / 8;
         for (int p = threadIdx.x; p < rows * per; p += 1024) {
             const int r = p / per, c = (p - r * per) * 8;
             v8 v = {};
@@ -604,7 +604,7 @@ unsigned at_most(int64_t want, int64_t most) { return (unsigned)(want < most ? w
 
 template <typename T>
 hipError_t fwd(const XentArgs &a, hipStream_t st) {
-    FA2_LAUNCH(xent_pack_kernel<T>, at_most(a.rows_pad / PACK_ROWS, 1024), 1024);
+    FA2_LAUNCH(xent_pack_kernel<T>, at_most(a.rows_pad / a.pack_rows, 1024), 1024);
     if (a.narrow)
         FA2_LAUNCH((xent_stats_kernel<T, XENT_NARROW_V / 64, 1, XENT_NARROW_V / 32, 256 / XENT_NARROW_V>), a.stat_items, 512);
     else

@@ -55,7 +55,6 @@ import os
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 from torch.compiler import is_compiling
 
 _THIS_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -330,72 +329,14 @@ def sdpa(query, key, value, attn_mask=None, dropout_p=0.0, is_causal=False, scal
 # ---------------------------------------------------------------------------
 # Operators on token rows (..., d)
 # ---------------------------------------------------------------------------
-_ROW_TYPES = (torch.float16, torch.bfloat16, torch.float32)
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-ROW_MAX = 16384   # FA2_ROW_MAX
-
-
-def _check_rows(name, x):
-    if not (x.is_cuda and x.dtype in _ROW_TYPES and x.dim() >= 1):
-        raise ValueError(f"{name} only supports fp16, bf16 and fp32 GPU tensors (..., d)")
-
-
-def _check_p(name, p):
-    if not 0.0 <= p < 1.0:
-        raise ValueError(f"{name}: dropout probability {p} outside [0, 1)")
-
-
-def _check_norm(name, x, residual, weight, eps, out_dtype):
-    _check_rows(name, x)
-    if not 1 <= x.shape[-1] <= ROW_MAX:
-        raise ValueError(f"{name}: rows of 1 to {ROW_MAX} elements, got {x.shape[-1]}")
-    if weight.shape != x.shape[-1:] or weight.dtype not in _ROW_TYPES or weight.device != x.device:
-        raise ValueError(f"{name}: weight must be ({x.shape[-1]},), fp16, bf16 or fp32, on x's device")
-    if residual is not None and (residual.shape != x.shape or residual.device != x.device
-                                 or residual.dtype not in (x.dtype, torch.float32)):
-        raise ValueError(f"{name}: residual must have x's shape and device, and x's type or fp32")
-    if out_dtype != x.dtype and (x.dtype != torch.float32 or out_dtype not in _ROW_TYPES):
-        raise ValueError(f"{name}: out_dtype must be x's type (fp16, bf16 or fp32 where x is fp32)")
-    if not 0.0 <= eps < float("inf"):
-        raise ValueError(f"{name}: eps {eps} is negative or not finite")
-
-
-class _RmsNorm(torch.autograd.Function):
-    """rms_norm (residual None: one output) and add_rms_norm (y, h).  Keeps h, which
-    the residual stream holds anyway, and one fp32 a row; the dropout mask is
-    formed again from the seed."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, eps, dropout_p, seed, out_dtype):
-        y, h, rstd = extension().rms_norm_fwd(x, residual, weight, eps, dropout_p, seed, out_dtype,
-                                              any(ctx.needs_input_grad))
-        ctx.save_for_backward(x if h is None else h, weight, rstd)
-        ctx.args = (x.dtype, dropout_p, seed)
-        ctx.set_materialize_grads(False)
-        return y if h is None else (y, h)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
-        if dy is None and dh is None:
-            return (None,) * 7
-        x_dtype, p, seed = ctx.args
-        want_x, want_r, want_w = ctx.needs_input_grad[:3]
-        if dy is None:   # only the stream's gradient: no norm in it
-            dx = (extension().dropout(dh, p, seed) if p > 0 else dh).to(x_dtype) if want_x else None
-            return dx, dh if want_r else None, torch.zeros_like(weight) if want_w else None, None, None, None, None
-        dx, dr, dw = extension().rms_norm_bwd(dy, dh, h, weight, rstd, x_dtype, p, seed, want_x, want_r, want_w)
-        return dx, dr, dw, None, None, None, None
 
 
 def rms_norm(x, weight, eps: float = 1e-6, out_dtype=None):
     """x * (mean(x^2) + eps)^-1/2 * weight over the last dimension, statistics in
     fp32 (the reference's FusedRMSNorm, train.py:1862-1875).  x (..., d) fp16,
     bf16 or fp32; ``out_dtype``: x's type, or any of these where x is fp32."""
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    _check_norm("rms_norm", x, None, weight, eps, out_dtype)
-    return _RmsNorm.apply(x, None, weight, float(eps), 0.0, 0, out_dtype)
+    return extension().rms_norm(x, weight, eps, out_dtype)
 
 
 def add_rms_norm(x, residual, weight, eps: float = 1e-6, dropout_p: float = 0.0, seed=None, out_dtype=None):
@@ -403,38 +344,16 @@ def add_rms_norm(x, residual, weight, eps: float = 1e-6, dropout_p: float = 0.0,
     ``y = rms_norm(h, weight, eps)``; returns ``(y, h)``.  residual: x's shape, x's
     type or fp32.  ``dropout_p`` > 0 drops elements of x by ``dropout``'s generator
     (``seed``: as there)."""
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if residual is None:
-        raise ValueError("add_rms_norm: residual is missing (rms_norm needs none)")
-    _check_norm("add_rms_norm", x, residual, weight, eps, out_dtype)
-    _check_p("add_rms_norm", dropout_p)
-    seed = _next_seed() if seed is None and dropout_p > 0 else int(seed or 0) & 0xFFFFFFFF
-    return _RmsNorm.apply(x, residual, weight, float(eps), float(dropout_p), seed, out_dtype)
+    if seed is None:
+        seed = _next_seed() if dropout_p and x.is_cuda else 0
+    return extension().add_rms_norm(x, residual, weight, eps, dropout_p, int(seed) & 0xFFFFFFFF, out_dtype)
 
 
 def rms_norm_fp8(x, weight, eps: float = 1e-6, residual=None):
     """The norm in 8 bits for a product that takes them, forward only: ``(q, scale)``,
     or ``(q, scale, h)`` with a residual; ``q * scale`` is the normalised row,
     q (..., d) float8_e4m3fn, scale (..., 1) fp32 = max(amax of the row / 448, 2^-126)."""
-    _check_norm("rms_norm_fp8", x, residual, weight, eps, x.dtype)
-    if _needs_grad(*(t for t in (x, weight, residual) if t is not None)):
-        raise RuntimeError("rms_norm_fp8 is inference-only (no backward)")
-    q, scale, h = extension().rms_norm_fp8(x, residual, weight, float(eps))
-    return (q, scale) if residual is None else (q, scale, h)
-
-
-class _Dropout(torch.autograd.Function):
-    """The gradient is the same call on dy with the same seed."""
-
-    @staticmethod
-    def forward(ctx, x, p, seed):
-        ctx.args = (p, seed)
-        return extension().dropout(x, p, seed)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        return extension().dropout(dy, *ctx.args), None, None
+    return extension().rms_norm_fp8(x, weight, eps, residual)
 
 
 def dropout(x, p: float, seed=None):
@@ -443,31 +362,9 @@ def dropout(x, p: float, seed=None):
     row = index of x flattened to (rows, d).  ``seed``: 32 bits; None takes the next
     one of the module's counter.  A captured graph keeps the seed it was captured
     with.  p = 0 returns x."""
-    _check_rows("dropout", x)
-    _check_p("dropout", p)
-    if p == 0.0:
-        return x
-    return _Dropout.apply(x, float(p), _next_seed() if seed is None else int(seed) & 0xFFFFFFFF)
-
-
-class _LinearCrossEntropy(torch.autograd.Function):
-    """Keeps the weight and the forward's state (log-sum-exp and packed states of the
-    tokens that count), no logits."""
-
-    @staticmethod
-    def forward(ctx, x, weight, target, ignore_index, reduction):
-        loss, state = extension().xent_fwd(x, weight, target, ignore_index, reduction)
-        ctx.save_for_backward(weight, state)
-        ctx.args = (x.shape, target.numel(), ignore_index, reduction)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dloss):
-        weight, state = ctx.saved_tensors
-        shape, rows, ignore_index, reduction = ctx.args
-        dx, dw = extension().xent_bwd(dloss, weight, state, rows, ignore_index, reduction, *ctx.needs_input_grad[:2])
-        return None if dx is None else dx.view(shape), dw, None, None, None
+    if seed is None:
+        seed = _next_seed() if x.is_cuda and p else 0
+    return extension().dropout(x, p, int(seed) & 0xFFFFFFFF)
 
 
 def linear_cross_entropy(x, weight, target, ignore_index: int = -100, reduction: str = "mean"):
@@ -478,17 +375,9 @@ def linear_cross_entropy(x, weight, target, ignore_index: int = -100, reduction:
     ``ignore_index`` (NaN if there is none), their sum, or with "none" one loss a
     token, 0 where ignored.  Ignored tokens cost nothing, and nothing in their
     states reaches loss or gradients.  A target outside the vocabulary gives NaN."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}")
     if torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
         x, weight = x.to(dtype), weight.to(dtype)
-    if not (x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1):
-        raise ValueError("linear_cross_entropy only supports fp16 and bf16 GPU tensors (..., d)")
-    if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or weight.dtype != x.dtype or weight.device != x.device:
-        raise ValueError("linear_cross_entropy: weight must be (V, d) of x's type, on x's device")
-    if not (1 <= weight.shape[1] <= ROW_MAX and 1 <= weight.shape[0] <= 1 << 24 and target.numel() <= 1 << 24):
-        raise ValueError(f"linear_cross_entropy: d of 1 to {ROW_MAX}, V of 1 to 2^24, at most 2^24 tokens")
-    if target.dtype != torch.int64 or target.shape != x.shape[:-1] or target.device != x.device:
-        raise ValueError("linear_cross_entropy: target must be int64 with x's leading dimensions, on x's device")
-    if reduction not in _REDUCTIONS:
-        raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}")
-    return _LinearCrossEntropy.apply(x, weight, target, int(ignore_index), _REDUCTIONS[reduction])
+    return extension().linear_cross_entropy(x, weight, target, ignore_index, _REDUCTIONS[reduction])
