@@ -320,7 +320,9 @@ typedef struct fa2_xent_params {
     int64_t ignore_index;
     float *loss;                         /* forward: [rows] (none), else [1]   */
     void *state;                         /* written by the forward, read by the
-                                            backward: fa2_xent_state_bytes     */
+                                            backward: fa2_xent_state_bytes.  NULL:
+                                            forward only; its workspace is then
+                                            larger by these bytes              */
     size_t state_bytes;
     const float *dloss;                  /* backward: gradient of loss         */
     int64_t dloss_stride;                /* none: elements between its rows    */

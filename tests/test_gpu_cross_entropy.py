@@ -264,3 +264,29 @@ def test_many_pieces_and_slices(fa):
 
 def test_large_vocabulary_few_tokens(fa):
     check(fa, *data(9, 128, 131072, BF16, 1))
+
+
+@pytest.mark.parametrize("n,d,V", [(1, 64, 1), (3, 64, 130), (64, 128, 4000), (65, 768, 16500), (199, 128, 20001), (256, 64, 32000),
+                                   (257, 64, 9000), (300, 192, 40000), (1000, 64, 33000), (5000, 64, 3001), (40, 100, 500)])
+@pytest.mark.parametrize("t", [F16, BF16])
+def test_forward_only(fa, n, d, V, t):
+    """Scoring: no gradient, one loss a token, states read where they are or packed; garbage in ignored tokens; a
+    strided and a misaligned view."""
+    x, w, target = data(n, d, V, t, n, ignored=0.2)
+    target[0] = V - 1
+    ref = run(fa, x, w, target, "none")[0]
+    z = x.double() @ w.double().T
+    S = (x.double().abs() @ w.double().abs().T).amax(1)
+    e = 2 * (d + 8) * 2.0 ** -24 * S + 2.0 ** -20 * (1 + z.abs().amax(1))
+    exact = torch.nn.functional.cross_entropy(z, target, reduction="none")
+    bad = x.clone()
+    bad[target == -100] = float("nan")
+    wide = torch.cat([bad, bad], 1)[:, :d]
+    off = torch.cat([bad.flatten()[:1], bad.flatten()])[1:].view(n, d)
+    with torch.no_grad():
+        for xx in (x, bad, wide, off):
+            got = fa.linear_cross_entropy(xx, w, target, reduction="none")
+            assert ((got.double() - exact).abs() <= e + 2.0 ** -23 * exact.abs()).all()
+            assert not got[target == -100].any()
+        total = fa.linear_cross_entropy(bad, w, target, reduction="sum")
+        assert abs(total.double() - ref.double().sum()) <= 2 * e.sum()

@@ -95,7 +95,8 @@ def _xent(lib, **kw):
     (dict(x=0), 1), (dict(weight=0), 1), (dict(target=0), 1), (dict(loss=0), 1),
     (dict(rows=(1 << 24) + 1), 2), (dict(hidden=0), 2), (dict(hidden=20000), 2), (dict(vocab=0), 2),
     (dict(weight_stride=64), 2), (dict(weight=BASE + 8), 3), (dict(weight_stride=132), 3), (dict(target=BASE + 4), 3),
-    (dict(type=capi.F32), 4), (dict(reduction=3), 4), (dict(state_bytes=100), 5), (dict(state=0), 5)])
+    (dict(type=capi.F32), 4), (dict(reduction=3), 4), (dict(state_bytes=100), 5),
+    (dict(state=0), 5)])   # without a state the workspace holds it too
 def test_cross_entropy_refusals(kw, status):
     lib = capi.load()
     ws = lib.fa2_xent_fwd_workspace_bytes(10, 128, 100)

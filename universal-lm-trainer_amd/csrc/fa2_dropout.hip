@@ -5,9 +5,10 @@
 // row and the column (fa2_device.h, head 0), so nothing but the seed is kept for
 // the gradient, which is the same kernel on dy.
 //
-// One pass, each thread eight elements of a row at a time (one 16-byte load of
-// fp16); a division finds its first row and column, later ones are found by
-// adding the grid's stride in rows and columns.
+// One pass, each thread a piece of E elements of a row at a time (eight, one 16-byte
+// load of fp16, where rows are made of such; else four, loaded by a type aligned to its
+// elements only, the last piece of a row by element); a division finds its first row
+// and column, later ones are found by adding the grid's stride in rows and columns.
 #include "fa2_token.h"
 
 namespace fa2 {
@@ -34,7 +35,10 @@ __global__ __launch_bounds__(256) void dropout_kernel(const DropoutArgs a) {
             for (int j = 0; j < 8; ++j) v[j] = drop(v[j], part, col + j, a.drop_thr, a.inv_keep);
             *reinterpret_cast<v8 *>(y) = __builtin_convertvector(v, v8);
         } else {
-            y[0] = (T)drop((float)x[0], part, col, a.drop_thr, a.inv_keep);
+            f4 v = load4(x, 0, a.cols - col, false);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = drop(v[j], part, col + j, a.drop_thr, a.inv_keep);
+            store4(y, 0, a.cols - col, false, v);
         }
         row += srow;
         c += sc;
@@ -47,13 +51,13 @@ __global__ __launch_bounds__(256) void dropout_kernel(const DropoutArgs a) {
 
 template <typename T>
 hipError_t run(const DropoutArgs &a, hipStream_t st) {
-    const uint64_t pieces = (uint64_t)a.rows * (a.vec ? a.cols / 8 : a.cols);
+    const uint64_t pieces = (uint64_t)a.rows * (a.vec ? a.cols / 8 : (a.cols + 3) / 4);
     const uint64_t want = (pieces + 255) / 256;
     const dim3 grid((unsigned)(want < 8192 ? want : 8192)), block(256);
     if (a.vec)
         hipLaunchKernelGGL((dropout_kernel<T, 8>), grid, block, 0, st, a);
     else
-        hipLaunchKernelGGL((dropout_kernel<T, 1>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((dropout_kernel<T, 4>), grid, block, 0, st, a);
     return hipGetLastError();
 }
 

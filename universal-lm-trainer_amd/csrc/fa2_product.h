@@ -1,5 +1,5 @@
 // fa2_product.h -- matrix product tiles, D[m, n] = sum_k A[m, k] B[n, k], on the
-// 32x32x16 MFMAs: operands by direct global->LDS transfers, two stages of 64 k.
+// 32x32x16 MFMAs: operands by direct global->LDS transfers, in stages of 64 k.
 //
 // Operands are 16-bit matrices in either order: ROWS are stored [m][k] (n for B),
 // the others [k][m].  A tile's operand is a number of panels of 64 x 64 elements (8
@@ -124,18 +124,18 @@ struct Frag {
     }
 };
 
-// Tile of 64 MP x 64 NP by eight waves in WM x WN, each (64 MP / WM) x (64 NP / WN).
-// APADDED: A has every row of the tile (B always has).
-template <typename T, bool AROWS, bool BROWS, bool APADDED, int MP, int NP, int WM, int WN>
+// Tile of 64 MP x 64 NP by eight waves in WM x WN, each (64 MP / WM) x (64 NP / WN),
+// with NS stages in LDS.  APADDED, BPADDED: A, B has every row of the tile.
+template <typename T, bool AROWS, bool BROWS, bool APADDED, bool BPADDED, int MP, int NP, int WM, int WN, int NS = 2>
 struct Product {
     static_assert(WM * WN == 8, "eight waves");
     static constexpr int TM = 64 * MP, TN = 64 * NP;
     static constexpr int MI = TM / WM / 32, NI = TN / WN / 32;   // a wave's 32x32 blocks
     static constexpr int STAGE = (MP + NP) * PANEL;
-    static constexpr int LDS = 2 * STAGE;
+    static constexpr int LDS = NS * STAGE;
 
     Feed<AROWS, APADDED, MP> A;
-    Feed<BROWS, true, NP> B;
+    Feed<BROWS, BPADDED, NP> B;
     Frag<T, AROWS> fa;
     Frag<T, BROWS> fb;
     char *mem;
@@ -152,8 +152,7 @@ struct Product {
         fb.init();
     }
 
-    // The stream of stages: `next` starts the transfers of the following stage, k0 of the
-    // operands, into the buffer that is free; stages are consumed in that order.
+    // Starts the transfers of stage k0 / PK into buffer buf.
     __device__ __forceinline__ void issue(int k0, int buf) const {
         A.issue(k0, lds + buf * STAGE);
         B.issue(k0, lds + buf * STAGE + MP * PANEL);
@@ -199,26 +198,37 @@ struct Product {
         }
     }
 
-    // A stream of stages.  begin() starts the first two and reads the first
+    // A stream of stages.  begin() starts the first NS and reads the first
     // fragments; steps() consumes n stages.  next(buf) starts the following stage's
-    // transfers into buffer buf, or nothing when there is none left.
+    // transfers into buffer buf and returns whether there was one left.
     //
     // The fragments of each k step are read while the step before is multiplied.
     // The one barrier of a stage stands before its last step: by then every wave
-    // holds that step's fragments, so the stage's buffer is free for the stage after
-    // the next, and the next stage has landed, so its first fragments can be read
+    // holds that step's fragments, so the stage's buffer is free for the stage NS
+    // later, and the next stage has landed, so its first fragments can be read
     // behind the last step's products.
     Frags f0;
-    int buf;
+    int buf, ahead;   // the current stage's buffer; stages started after it
 
     template <typename N>
     __device__ __forceinline__ void begin(N next) {
-        next(0);
-        next(1);
-        vm_wait<0>();
-        lds_barrier();
+        ahead = -1;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) ahead += next(s) ? 1 : 0;
+        landed<NS - 1>();
         buf = 0;
         read(f0, 0, 0);
+    }
+
+    // Every wave's transfers of all but the last `F` stages started have landed, if all
+    // those are under way (a wave's loads complete in order); else all of them.
+    template <int F>
+    __device__ __forceinline__ void landed() const {
+        if (F > 0 && ahead == F)
+            vm_wait<F *(MP + NP)>();
+        else
+            vm_wait<0>();
+        lds_barrier();
     }
 
     template <typename N>
@@ -234,10 +244,10 @@ struct Product {
             read(f1, buf, 3);
             multiply(f0, acc);
             interleave();
-            vm_wait<0>();
-            lds_barrier();
-            next(buf);
-            buf ^= 1;
+            --ahead;   // from the next stage on
+            landed<NS - 2>();
+            ahead += next(buf) ? 1 : 0;
+            buf = NS == 2 ? buf ^ 1 : buf == NS - 1 ? 0 : buf + 1;
             read(f0, buf, 0);
             multiply(f1, acc);
             interleave();
@@ -251,8 +261,10 @@ struct Product {
         if (kbeg >= kend) return;
         int k = kbeg;
         auto next = [&](int b) FA2_INLINE {
-            if (k < kend) issue(k, b);
+            if (k >= kend) return false;
+            issue(k, b);
             k += PK;
+            return true;
         };
         begin(next);
         steps((kend - kbeg) / PK, acc, next);

@@ -80,7 +80,24 @@ struct DropoutArgs {
 // are `rows_pad` (a multiple of XENT_PAD) with zeros behind the last one.
 constexpr int XENT_PAD = 256;      // packed rows and a piece's columns: multiples of this
 constexpr int XENT_KPAD = 64;      // the hidden size the products see: a multiple of this
-constexpr int XENT_NARROW_V = 128; // vocabulary rows of the forward's tiles of 64 tokens
+
+// Slices of the vocabulary for the forward over n tokens: the workgroups (token tiles x
+// slices) fill the slots once, or a few times where that leaves fewer of them idle; the
+// cost of a choice is its rounds times the tiles of a slice.
+__host__ __device__ inline int xent_stat_splits(int tile_n, int tile_m, int slots, int rounds, int n, int V) {
+    const int rt = n > tile_n ? (n + tile_n - 1) / tile_n : 1, tiles = (V + tile_m - 1) / tile_m;
+    int best = 1, cost = INT32_MAX;
+    for (int k = 1; k <= rounds; ++k) {
+        int s = k * slots / rt;
+        s = s < 1 ? 1 : s > tiles ? tiles : s;
+        const int c = (rt * s + slots - 1) / slots * ((tiles + s - 1) / s);
+        if (c < cost) {
+            cost = c;
+            best = s;
+        }
+    }
+    return best;
+}
 
 struct XentArgs {
     int64_t rows;                  // N
@@ -101,11 +118,14 @@ struct XentArgs {
     int *rowmap;                   // [rows_pad]
     int *tgt;                      // [rows_pad]: target, -1 where it is outside the vocabulary
     float *lse;                    // [rows_pad]
-    void *xc;                      // [rows_pad, dp]
+    void *xc;                      // [rows_pad, dp]; direct: the states themselves
+    int64_t xc_stride;
     // forward
     int pack_rows;                 // packed rows a workgroup has at a time
-    bool narrow;                   // tiles of 64 tokens, not 256
+    bool direct;                   // nothing is packed: every token is a row, nothing is kept
+    int stat_tile_n, stat_tile_m;  // tokens and vocabulary rows of a tile
     int stat_slots, stat_rounds;   // workgroups resident at once; rounds of them to consider
+    int stat_splits;               // direct: slices of the vocabulary
     int stat_items;                // workgroups there are partial results for
     float *part;                   // [token][slice] (maximum, sum)
     float *row_loss;               // sum, mean: [N]
@@ -148,16 +168,21 @@ __device__ __forceinline__ float drop(float v, uint32_t part_row, int col, uint3
     return dropout_keep_hashed(part_row ^ dropout_col_term(col), thr) ? v * inv_keep : 0.f;
 }
 
-// Four elements of a row from column col on, as fp32; zero past the row's end.
+// Four elements of a row from column col on, as fp32; zero past the row's end.  vec:
+// rows and width are multiples of four elements; else whole groups of four are still
+// one load, of a type aligned to its elements only (global memory takes it).
 template <typename T>
 __device__ __forceinline__ f4 load4(const T *row, int col, int cols, bool vec) {
+    typedef typename vec_of<T>::v4 v4;
+    typedef T u4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
     f4 r = {0.f, 0.f, 0.f, 0.f};
     if (vec) {
-        if (col < cols)
-            r = __builtin_convertvector(*reinterpret_cast<const typename vec_of<T>::v4 *>(row + col), f4);
+        if (col < cols) r = __builtin_convertvector(*reinterpret_cast<const v4 *>(row + col), f4);
+    } else if (col + 4 <= cols) {
+        r = __builtin_convertvector((v4)*reinterpret_cast<const u4 *>(row + col), f4);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 3; ++j)
             if (col + j < cols) r[j] = (float)row[col + j];
     }
     return r;
@@ -165,12 +190,16 @@ __device__ __forceinline__ f4 load4(const T *row, int col, int cols, bool vec) {
 
 template <typename T>
 __device__ __forceinline__ void store4(T *row, int col, int cols, bool vec, f4 v) {
-    const typename vec_of<T>::v4 q = __builtin_convertvector(v, typename vec_of<T>::v4);
+    typedef typename vec_of<T>::v4 v4;
+    typedef T u4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    const v4 q = __builtin_convertvector(v, v4);
     if (vec) {
-        if (col < cols) *reinterpret_cast<typename vec_of<T>::v4 *>(row + col) = q;
+        if (col < cols) *reinterpret_cast<v4 *>(row + col) = q;
+    } else if (col + 4 <= cols) {
+        *reinterpret_cast<u4 *>(row + col) = q;
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 3; ++j)
             if (col + j < cols) row[col + j] = q[j];
     }
 }

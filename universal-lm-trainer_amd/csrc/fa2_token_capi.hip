@@ -67,8 +67,8 @@ int check_norm_types(int x, int res, int y, bool fp8) {
 // ---------------------------------------------------------------------------
 struct XentPlan {
     int rows_pad, dp;
-    bool narrow, small;
-    int stat_slots, stat_rounds, stat_items;
+    bool small;
+    int stat_tile_n, stat_tile_m, stat_slots, stat_rounds, stat_items;
     int slots, piece, pieces, strip, xcap;
     int wsplit, wsplit_last;
     // offsets in the state
@@ -89,13 +89,16 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     p.rows_pad = (int)((rows + XENT_PAD - 1) / XENT_PAD * XENT_PAD);
     p.dp = (d + XENT_KPAD - 1) / XENT_KPAD * XENT_KPAD;
     const int64_t R = p.rows_pad;
-    // Forward.  Up to 1024 tokens in tiles of 64, three workgroups a compute unit; else of 256, one.
-    p.narrow = R <= 1024;
-    p.stat_slots = p.narrow ? 768 : 256;
-    p.stat_rounds = p.narrow ? 1 : 4;
-    const int64_t token_tiles = p.narrow ? (rows + 63) / 64 : R / 256;
+    // Forward: tiles of 256 tokens x 256 vocabulary rows, one workgroup a compute unit;
+    // where those are fewer than two a unit, 256 x 128 (and a deeper stream of stages); up
+    // to 64 tokens, and where even these leave half the units idle, 64 x 128, two a unit.
+    const int64_t t256 = R / 256, v256 = (V + 255) / 256, v128 = (V + 127) / 128;
+    p.stat_tile_m = t256 * v256 < 512 ? 128 : 256;
+    p.stat_tile_n = p.stat_tile_m == 128 && (rows <= 64 || t256 * v128 < 128) ? 64 : 256;
+    p.stat_slots = p.stat_tile_n == 64 ? 512 : 256;
+    p.stat_rounds = p.stat_tile_m == 256 ? 4 : 2;
+    const int64_t token_tiles = (rows + p.stat_tile_n - 1) / p.stat_tile_n, v_tiles = p.stat_tile_m == 256 ? v256 : v128;
     p.stat_items = (int)(token_tiles > p.stat_slots * p.stat_rounds ? token_tiles : p.stat_slots * p.stat_rounds);
-    const int64_t v_tiles = (V + (p.narrow ? XENT_NARROW_V : 256) - 1) / (p.narrow ? XENT_NARROW_V : 256);
     if (p.stat_items > token_tiles * v_tiles) p.stat_items = (int)(token_tiles * v_tiles);
     // Backward.  A piece's P is at most 256 MiB (twice, with more than one piece), in equal pieces.
     const int64_t most = clamp(((int64_t)256 << 20) / (2 * R) / XENT_PAD * XENT_PAD, XENT_PAD, 1 << 24);
@@ -129,7 +132,7 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     const size_t wbytes = d % XENT_KPAD ? (size_t)V * p.dp * 2 : 0;
     at = 0;
     p.f_weight = take(wbytes);
-    p.part = take((size_t)p.stat_items * (p.narrow ? 64 : 256) * 8);
+    p.part = take((size_t)p.stat_items * p.stat_tile_n * 8);
     p.row_loss = take((size_t)rows * 4);
     p.fwd_bytes = at;
     at = 0;
@@ -167,19 +170,19 @@ int xent_check(const fa2_xent_params *p, const void *ws, size_t ws_bytes, bool b
         if (!backward && !aligned(p->target, 8)) return fail(FA2_ERR_MISALIGNED, "target is not 8-byte aligned");
     }
     const size_t state = fa2_xent_state_bytes(p->rows, p->hidden);
-    if (!p->state || p->state_bytes < state)
+    const bool keeps = backward || p->state;
+    if (keeps && (!p->state || p->state_bytes < state))
         return fail(FA2_ERR_WORKSPACE, "state needs %zu bytes, got %zu", state, p->state ? p->state_bytes : 0);
     const size_t need = backward ? fa2_xent_bwd_workspace_bytes(p->rows, p->hidden, p->vocab)
-                                 : fa2_xent_fwd_workspace_bytes(p->rows, p->hidden, p->vocab);
+                                 : fa2_xent_fwd_workspace_bytes(p->rows, p->hidden, p->vocab) + (keeps ? 0 : state);
     if (!ws || ws_bytes < need) return fail(FA2_ERR_WORKSPACE, "workspace needs %zu bytes, got %zu", need, ws ? ws_bytes : 0);
     if (!aligned(ws, 16) || !aligned(p->state, 16)) return fail(FA2_ERR_MISALIGNED, "state and workspace must be 16-byte aligned");
     return FA2_OK;
 }
 
-fa2::XentArgs xent_args(const fa2_xent_params *p, const XentPlan &pl) {
+fa2::XentArgs xent_args(const fa2_xent_params *p, const XentPlan &pl, char *s) {
     fa2::XentArgs a;
     memset(&a, 0, sizeof(a));
-    char *s = static_cast<char *>(p->state);
     a.rows = p->rows;
     a.rows_pad = pl.rows_pad;
     a.d = p->hidden;
@@ -199,8 +202,10 @@ fa2::XentArgs xent_args(const fa2_xent_params *p, const XentPlan &pl) {
     a.rowmap = reinterpret_cast<int *>(s + pl.rowmap);
     a.pos = reinterpret_cast<int *>(s + pl.pos);
     a.xc = s + pl.xc;
+    a.xc_stride = pl.dp;
     a.pack_rows = pl.rows_pad <= 4096 ? 16 : 64;
-    a.narrow = pl.narrow;
+    a.stat_tile_n = pl.stat_tile_n;
+    a.stat_tile_m = pl.stat_tile_m;
     a.stat_slots = pl.stat_slots;
     a.stat_rounds = pl.stat_rounds;
     a.stat_items = pl.stat_items;
@@ -338,9 +343,18 @@ int fa2_xent_fwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
     if (!p->loss && !(p->rows == 0 && p->reduction == FA2_REDUCE_NONE)) return fail(FA2_ERR_NULL_POINTER, "loss is NULL");
     if (!aligned(p->loss, 4)) return fail(FA2_ERR_MISALIGNED, "loss is not 4-byte aligned");
     const XentPlan pl = xent_plan(p->rows > 0 ? p->rows : 1, p->hidden, p->vocab);
-    fa2::XentArgs a = xent_args(p, pl);
     char *w = static_cast<char *>(workspace);
+    fa2::XentArgs a = xent_args(p, pl, p->state ? static_cast<char *>(p->state) : w + pl.fwd_bytes);
     const hipStream_t st = (hipStream_t)stream;
+    // Nothing kept, and states that the products can read: few enough tokens are not
+    // packed (the weights' bytes, not the tokens, set the time), which saves a launch.
+    a.direct = !p->state && p->reduction == FA2_REDUCE_NONE && pl.stat_tile_m == 128 && p->rows > 0 &&
+               p->hidden % fa2::XENT_KPAD == 0 && aligned(p->x, 16) && p->x_stride % 8 == 0 && p->x_stride < 1 << 22;
+    if (a.direct) {
+        a.xc = const_cast<void *>(p->x);
+        a.xc_stride = p->x_stride;
+        a.stat_splits = fa2::xent_stat_splits(a.stat_tile_n, a.stat_tile_m, a.stat_slots, a.stat_rounds, (int)p->rows, a.V);
+    }
     a.part = reinterpret_cast<float *>(w + pl.part);
     a.row_loss = reinterpret_cast<float *>(w + pl.row_loss);
     a.loss = p->loss;
@@ -366,7 +380,7 @@ int fa2_xent_bwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
     if (p->dloss_stride < 0 || p->dloss_stride > INT32_MAX) return fail(FA2_ERR_BAD_SHAPE, "dloss stride %lld outside 0 .. 2^31 - 1", (long long)p->dloss_stride);
     if (!aligned(p->dx, 16) || !aligned(p->dweight, 16)) return fail(FA2_ERR_MISALIGNED, "dx and dweight must be 16-byte aligned");
     const XentPlan pl = xent_plan(p->rows > 0 ? p->rows : 1, p->hidden, p->vocab);
-    fa2::XentArgs a = xent_args(p, pl);
+    fa2::XentArgs a = xent_args(p, pl, static_cast<char *>(p->state));
     char *w = static_cast<char *>(workspace);
     const hipStream_t st = (hipStream_t)stream;
     a.g = p->dloss;

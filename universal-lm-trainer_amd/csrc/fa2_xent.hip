@@ -37,24 +37,6 @@ enum { N_TOKENS = 0, STAT_SPLITS = 1 };
 // Packing
 // ---------------------------------------------------------------------------
 
-// Slices of the vocabulary for the forward: the workgroups (token tiles x slices)
-// fill the slots once, or a few times where that leaves fewer of them idle; the
-// cost of a choice is its rounds times the tiles of a slice.
-__device__ __forceinline__ int stat_splits(const XentArgs &a, int n) {
-    const int tm = a.narrow ? XENT_NARROW_V : 256, rt = max(1, (n + (a.narrow ? 64 : 256) - 1) / (a.narrow ? 64 : 256));
-    const int tiles = (a.V + tm - 1) / tm;
-    int best = 1, cost = INT32_MAX;
-    for (int k = 1; k <= a.stat_rounds; ++k) {
-        const int s = max(1, min(tiles, k * a.stat_slots / rt));
-        const int c = (rt * s + a.stat_slots - 1) / a.stat_slots * ((tiles + s - 1) / s);
-        if (c < cost) {
-            cost = c;
-            best = s;
-        }
-    }
-    return best;
-}
-
 constexpr int PACK_ROWS = 64;   // packed rows a workgroup has at a time, at most
 
 // Every workgroup counts through all targets, and does its share of the rest: the
@@ -67,7 +49,8 @@ __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
     typedef typename vec_of<T>::v8 v8;
     constexpr int Q = 16;   // targets a thread has at a time
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t i0 = a.rows * blockIdx.x / gridDim.x, i1 = a.rows * (blockIdx.x + 1) / gridDim.x;
+    const int share = ((int)a.rows + gridDim.x - 1) / gridDim.x;   // of the tokens' packed rows (at most 2^24 tokens)
+    const int64_t i0 = (int64_t)blockIdx.x * share, i1 = min(a.rows, i0 + share);
     const bool vec = a.x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.d % 8 == 0;
     for (int j0 = blockIdx.x * a.pack_rows; j0 < a.rows_pad; j0 += gridDim.x * a.pack_rows) {
         int n = 0;   // tokens that count so far
@@ -108,7 +91,7 @@ __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
         }
         if (j0 == 0 && threadIdx.x == 0) {
             a.count[N_TOKENS] = n;
-            a.count[STAT_SPLITS] = stat_splits(a, n);
+            a.count[STAT_SPLITS] = xent_stat_splits(a.stat_tile_n, a.stat_tile_m, a.stat_slots, a.stat_rounds, n, a.V);
         }
         if ((int)threadIdx.x < a.pack_rows && j0 + (int)threadIdx.x >= n) a.tgt[j0 + threadIdx.x] = -1;
         __syncthreads();
@@ -165,12 +148,12 @@ __device__ __forceinline__ void join_max_sum(float &m, float &l, float m2, float
 // the maximum of the lane's first tile and moves only when a sum passes 2^100: fp32
 // holds the terms of any larger logits until then.  The slice's tiles are one stream
 // of stages: the next tile's transfers run behind the exponentials.
-template <typename T, int MP, int NP, int WM, int WN>
+template <typename T, int MP, int NP, int WM, int WN, int NS>
 __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
-    typedef Product<T, true, true, false, MP, NP, WM, WN> Pr;
+    typedef Product<T, true, true, false, MP == 4, MP, NP, WM, WN, NS> Pr;   // MP < 4: the states may be the caller's
     constexpr int MI = Pr::MI, NI = Pr::NI;
     __shared__ __align__(16) char mem[Pr::LDS];
-    const int n = a.count[N_TOKENS], splits = a.count[STAT_SPLITS];
+    const int n = a.direct ? (int)a.rows : a.count[N_TOKENS], splits = a.direct ? a.stat_splits : a.count[STAT_SPLITS];
     const int rt = (n + Pr::TN - 1) / Pr::TN;
     if ((int)blockIdx.x >= rt * splits) return;
     // groups of 8 token tiles, in a group the tokens fastest: a slice's weights meet in one XCD's L2
@@ -182,7 +165,7 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
     Pr pr;
     pr.init(mem);
     pr.A.init(a.w, a.w_stride, t0 * Pr::TM, a.V, 0);
-    pr.B.init(a.xc, a.dp, rb * Pr::TN, a.rows_pad, 0);
+    pr.B.init(a.xc, a.xc_stride, rb * Pr::TN, a.direct ? n : a.rows_pad, 0);
     float ref[NI], sum[NI];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
@@ -191,13 +174,14 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
     }
     int nt = t0, nk = 0;   // tile and k of the next stage
     auto next = [&](int buf) FA2_INLINE {
-        if (nt >= t1) return;
+        if (nt >= t1) return false;
         pr.issue(nk, buf);
         nk += PK;
         if (nk == a.dp) {
             nk = 0;
             if (++nt < t1) pr.A.init(a.w, a.w_stride, nt * Pr::TM, a.V, 0);
         }
+        return true;
     };
     pr.begin(next);
     for (int t = t0; t < t1; ++t) {
@@ -272,15 +256,16 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
 // own (found among the tiles' logits it cost the forward's kernel 6%).
 template <typename T>
 __global__ __launch_bounds__(256) void xent_join_kernel(const XentArgs a) {
-    const int lane = threadIdx.x & 63, splits = a.count[STAT_SPLITS];
+    const int lane = threadIdx.x & 63, splits = a.direct ? a.stat_splits : a.count[STAT_SPLITS];
     const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= a.rows) return;
-    const int j = a.pos[i];
+    const int64_t target = a.target[i];
+    const int j = target == a.ignore ? -1 : a.direct ? (int)i : a.pos[i];
     float loss = 0.f;
     if (j >= 0) {
-        const int t = a.tgt[j];
+        const int t = target >= 0 && target < a.V ? (int)target : -1;
         typedef typename vec_of<T>::v8 v8;
-        const T *x = static_cast<const T *>(a.xc) + (int64_t)j * a.dp;
+        const T *x = static_cast<const T *>(a.xc) + (int64_t)j * a.xc_stride;
         const T *w = static_cast<const T *>(a.w) + (int64_t)max(t, 0) * a.w_stride;
         float z = 0.f;
         for (int c = lane * 8; c < a.dp; c += 512) {
@@ -301,7 +286,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const XentArgs a) {
         }
         const float lse = m + logf(l);
         loss = t >= 0 ? lse - z : NAN;   // a target outside the vocabulary
-        if (lane == 0) a.lse[j] = lse;
+        if (lane == 0 && !a.direct) a.lse[j] = lse;
     }
     if (lane == 0) (a.reduction == FA2_REDUCE_NONE ? a.loss : a.row_loss)[i] = loss;
 }
@@ -386,7 +371,7 @@ __device__ __forceinline__ XentWork xent_work(const XentArgs &a, int n) {
 // vocabulary rows, N side tokens.  In units of 1 / P_SCALE, times the row's factor.
 template <typename T, int MP>
 __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k, int item, int n, char *mem, char *out) {
-    typedef Product<T, true, true, false, MP, MP, 2, 4> Pr;
+    typedef Product<T, true, true, false, true, MP, MP, 2, 4> Pr;
     const int tiles = (a.p1 - a.p0 + Pr::TM - 1) / Pr::TM, strips = (tiles + a.strip - 1) / a.strip;
     // groups of 8 token tiles, in a group the tokens fastest
     const int g = item / (8 * strips), gs = min(8, k.rt - 8 * g), in = item - g * 8 * strips;
@@ -408,13 +393,14 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
     }
     int nt = t0, nk = 0;
     auto next = [&](int buf) FA2_INLINE {
-        if (nt >= t1) return;
+        if (nt >= t1) return false;
         pr.issue(nk, buf);
         nk += PK;
         if (nk == a.dp) {
             nk = 0;
             if (++nt < t1) pr.A.init(a.w, a.w_stride, a.p0 + nt * Pr::TM, a.V, 0);
         }
+        return true;
     };
     pr.begin(next);
     char *blk = out + (threadIdx.x >> 6) * 4096;
@@ -456,7 +442,7 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
 // vocabulary rows, K packed tokens.
 template <typename T, int MP>
 __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n, char *mem) {
-    typedef Product<T, false, false, true, MP, MP, 2, 4> Pr;
+    typedef Product<T, false, false, true, true, MP, MP, 2, 4> Pr;
     const int nd = (a.d + Pr::TM - 1) / Pr::TM, nv = (a.v1 - a.v0 + Pr::TM - 1) / Pr::TM;
     const int db = item % nd, vb = item / nd % nv, s = item / nd / nv;
     const int kt = (n + Pr::TM - 1) / Pr::TM * MP;
@@ -500,7 +486,7 @@ __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n,
 // side hidden columns, K the piece.
 template <typename T, int MP>
 __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &k, int item, char *mem) {
-    typedef Product<T, true, false, true, MP, MP, 2, 4> Pr;
+    typedef Product<T, true, false, true, true, MP, MP, 2, 4> Pr;
     const int nd = (a.d + Pr::TN - 1) / Pr::TN;
     const int db = item % nd, rb = item / nd % k.rt, s = item / nd / k.rt;
     const int kt = (a.v1 - a.v0 + PK - 1) / PK;
@@ -533,7 +519,7 @@ __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &
 // an item, whose output goes through the panels.
 template <typename T, int MP>
 __global__ __launch_bounds__(512, 2) void xent_grad_kernel(const XentArgs a) {
-    constexpr int PANELS = Product<T, true, true, false, MP, MP, 2, 4>::LDS;
+    constexpr int PANELS = Product<T, true, true, false, true, MP, MP, 2, 4>::LDS;
     __shared__ __align__(16) char mem[PANELS + (MP == 4 ? 8 * 4096 : 0)];
     const int n = a.count[N_TOKENS];
     const XentWork k = xent_work<MP>(a, n);
@@ -604,11 +590,13 @@ unsigned at_most(int64_t want, int64_t most) { return (unsigned)(want < most ? w
 
 template <typename T>
 hipError_t fwd(const XentArgs &a, hipStream_t st) {
-    FA2_LAUNCH(xent_pack_kernel<T>, at_most(a.rows_pad / a.pack_rows, 1024), 1024);
-    if (a.narrow)
-        FA2_LAUNCH((xent_stats_kernel<T, XENT_NARROW_V / 64, 1, XENT_NARROW_V / 32, 256 / XENT_NARROW_V>), a.stat_items, 512);
+    if (!a.direct) FA2_LAUNCH(xent_pack_kernel<T>, at_most(a.rows_pad / a.pack_rows, 1024), 1024);
+    if (a.stat_tile_n == 64)
+        FA2_LAUNCH((xent_stats_kernel<T, 2, 1, 4, 2, 3>), a.stat_items, 512);
+    else if (a.stat_tile_m == 128)
+        FA2_LAUNCH((xent_stats_kernel<T, 2, 4, 2, 4, 3>), a.stat_items, 512);
     else
-        FA2_LAUNCH((xent_stats_kernel<T, 4, 4, 2, 4>), a.stat_items, 512);
+        FA2_LAUNCH((xent_stats_kernel<T, 4, 4, 2, 4, 2>), a.stat_items, 512);
     if (a.rows > 0) FA2_LAUNCH(xent_join_kernel<T>, (unsigned)((a.rows + 3) / 4), 256);
     if (a.reduction != FA2_REDUCE_NONE) FA2_LAUNCH(xent_sum_kernel, 1, 1024);
     return hipSuccess;

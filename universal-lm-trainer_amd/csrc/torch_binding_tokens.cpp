@@ -341,7 +341,7 @@ struct XentOut {
     Tensor loss, state;
 };
 
-XentOut xent_run(const Tensor &x, const Tensor &w, const Tensor &target, int64_t ignore_index, int64_t reduction) {
+XentOut xent_run(const Tensor &x, const Tensor &w, const Tensor &target, int64_t ignore_index, int64_t reduction, bool keep) {
     const char *op = "linear_cross_entropy";
     at::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     const int64_t rows = target.numel();
@@ -356,10 +356,14 @@ XentOut xent_run(const Tensor &x, const Tensor &w, const Tensor &target, int64_t
     q.weight_stride = wr.stride(0);
     q.target = tc.data_ptr<int64_t>();
     q.loss = loss.data_ptr<float>();
-    q.state_bytes = fa2_xent_state_bytes(rows, q.hidden);
-    Tensor state = bytes_of(q.state_bytes, x);
-    q.state = state.data_ptr();
-    const size_t bytes = fa2_xent_fwd_workspace_bytes(rows, q.hidden, q.vocab);
+    const size_t state_bytes = fa2_xent_state_bytes(rows, q.hidden);
+    Tensor state;
+    if (keep) {
+        state = bytes_of(state_bytes, x);
+        q.state = state.data_ptr();
+        q.state_bytes = state_bytes;
+    }
+    const size_t bytes = fa2_xent_fwd_workspace_bytes(rows, q.hidden, q.vocab) + (keep ? 0 : state_bytes);
     const Tensor ws = bytes_of(bytes, x);
     check_rc(fa2_xent_fwd(&q, ws.data_ptr(), bytes, stream_of(x)), op);
     return {loss, state};
@@ -393,7 +397,7 @@ std::tuple<Tensor, Tensor> xent_grads(const Tensor &dloss, const Tensor &w, cons
 struct XentFn : torch::autograd::Function<XentFn> {
     static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const Tensor &target, int64_t ignore_index,
                           int64_t reduction) {
-        const XentOut o = xent_run(x, w, target, ignore_index, reduction);
+        const XentOut o = xent_run(x, w, target, ignore_index, reduction, true);
         ctx->save_for_backward({w, o.state});
         ctx->saved_data["shape"] = x.sizes().vec();
         ctx->saved_data["ignore"] = ignore_index;
@@ -414,7 +418,7 @@ struct XentFn : torch::autograd::Function<XentFn> {
 Tensor linear_cross_entropy(const Tensor &x, const Tensor &w, const Tensor &target, int64_t ignore_index, int64_t reduction) {
     check_xent(x, w, target, "linear_cross_entropy");
     if (wants_grad(x) || wants_grad(w)) return XentFn::apply(x, w, target, ignore_index, reduction);
-    return xent_run(x, w, target, ignore_index, reduction).loss;
+    return xent_run(x, w, target, ignore_index, reduction, false).loss;
 }
 
 }  // namespace
