@@ -225,7 +225,7 @@ int fa2_rope_f16(const fa2_rope_params *p, int32_t backward, void *stream);
 enum fa2_dtype { FA2_F16 = 0, FA2_BF16 = 1, FA2_F32 = 2, FA2_E4M3 = 3 /* OCP 8-bit: 4 exponent, 3 mantissa bits */ };
 
 /* Largest row fa2_rms_norm_* and the largest hidden size fa2_xent_* take. */
-#define FA2_ROW_MAX 16384
+#define FA2_ROW_MAX 8192
 
 /* RMS norm with the residual's addition (reference @ None: train.py:1862-1875 and
  * the additions of train.py:1986-1994, there separate torch calls):

@@ -90,7 +90,7 @@ def check_all(fa, x, r, w, dy, dh, eps, p=0.0, seed=7, rows_of=None):
 
 
 @pytest.mark.parametrize("cols", [1, 2, 3, 4, 63, 64, 65, 255, 256, 257, 512, 768, 771, 1000, 1024, 1025, 2048, 2049, 4096,
-                                  4100, 8192, 16383, 16384])
+                                  4100, 6000, 8191, 8192])
 @pytest.mark.parametrize("xt,rt", [(F16, F32), (BF16, BF16)])
 def test_widths(fa, cols, xt, rt):
     check_all(fa, *data(5, cols, xt, rt, rt, cols), eps=1e-6, p=0.1)
@@ -214,7 +214,7 @@ def e4m3(v):
     return torch.round(v / step) * step
 
 
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 768), (8, 768), (5, 771), (3, 1025), (2, 5000), (1, 16384), (300, 256)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 768), (8, 768), (5, 771), (3, 1025), (2, 5000), (1, 8192), (300, 256)])
 @pytest.mark.parametrize("xt,rt", [(F16, F16), (BF16, F32), (F32, F32), (F16, None), (F32, None)])
 def test_fp8(fa, rows, cols, xt, rt):
     x, r, w, _, _ = data(rows, cols, xt, rt or F32, F32, rows + cols)
@@ -254,7 +254,7 @@ def test_refusals_on_gpu(fa):
                  lambda: fa.add_rms_norm(x, r[:2], w), lambda: fa.add_rms_norm(x, r.bfloat16(), w),
                  lambda: fa.add_rms_norm(x, None, w), lambda: fa.add_rms_norm(x, r, w, dropout_p=1.0),
                  lambda: fa.rms_norm(x, w, out_dtype=F32), lambda: fa.rms_norm(x, w, eps=-1.0),
-                 lambda: fa.rms_norm(torch.zeros(2, 16385, device=DEV), torch.zeros(16385, device=DEV))):
+                 lambda: fa.rms_norm(torch.zeros(2, 8193, device=DEV), torch.zeros(8193, device=DEV))):
         with pytest.raises(ValueError):
             call()
     with pytest.raises(RuntimeError):

@@ -240,7 +240,6 @@ hipError_t by_cols(int cols, F f) {
     FA2_COLS(256, 3);
     FA2_COLS(256, 4);
     FA2_COLS(1024, 2);
-    FA2_COLS(1024, 4);
 #undef FA2_COLS
     return hipErrorInvalidValue;
 }

@@ -88,13 +88,14 @@ struct Feed {
 };
 
 // Fragment reads of one operand: 32 rows (columns) from `at` (a multiple of 32) of
-// the tile, k step ks of the stage.
-template <typename T, bool ROWS>
+// the tile, k step ks of the stage.  W: rows (columns) that a wave reads in all.
+template <typename T, bool ROWS, int W>
 struct Frag {
     typedef typename vec_of<T>::v8 v8;
     uint32_t off[4];   // ROWS: of k step 0..3; else: column 0 / 32 of a panel, first / second read
 
-    __device__ __forceinline__ void init() {
+    // first: the first row (column) that the wave reads.
+    __device__ __forceinline__ void init(int first) {
         const int lane = threadIdx.x & 63;
         if constexpr (ROWS) {
             const int c = lane & 31, g2 = lane >> 5;
@@ -103,8 +104,9 @@ struct Frag {
         } else {
             const int G = lane >> 4, s = lane & 15;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = 8 * (G >> 1) + (s >> 2) + 4 * (q & 1), col = 32 * (q >> 1) + 16 * (G & 1) + 4 * (s & 3);
+            for (int q = 0; q < (W == 32 ? 2 : 4); ++q) {
+                const int half = W == 32 ? first & 32 : 32 * (q >> 1);
+                const int row = 8 * (G >> 1) + (s >> 2) + 4 * (q & 1), col = half + 16 * (G & 1) + 4 * (s & 3);
                 off[q] = (uint32_t)(row * 128 + (((col >> 3) ^ swz_tr(row)) << 4) + 2 * (col & 7));
             }
         }
@@ -116,7 +118,7 @@ struct Frag {
         if constexpr (ROWS) {
             return *(__attribute__((address_space(3))) const v8 *)(p + (at & 32) * 128 + off[ks]);
         } else {
-            const int q = (at & 32) >> 4;
+            const int q = W == 32 ? 0 : (at & 32) >> 4;
             const s4v r0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v *)(p + ks * 2048 + off[q]));
             const s4v r1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v *)(p + ks * 2048 + off[q + 1]));
             return __builtin_bit_cast(v8, __builtin_shufflevector(r0, r1, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -136,8 +138,8 @@ struct Product {
 
     Feed<AROWS, APADDED, MP> A;
     Feed<BROWS, BPADDED, NP> B;
-    Frag<T, AROWS> fa;
-    Frag<T, BROWS> fb;
+    Frag<T, AROWS, TM / WM> fa;
+    Frag<T, BROWS, TN / WN> fb;
     char *mem;
     uint32_t lds;
     int wm, wn;        // the wave's first row and column of the tile
@@ -148,8 +150,8 @@ struct Product {
         lds = lds_addr(m);
         wm = (w % WM) * (TM / WM);
         wn = (w / WM) * (TN / WN);
-        fa.init();
-        fb.init();
+        fa.init(wm);
+        fb.init(wn);
     }
 
     // Starts the transfers of stage k0 / PK into buffer buf.
@@ -207,23 +209,26 @@ struct Product {
     // holds that step's fragments, so the stage's buffer is free for the stage NS
     // later, and the next stage has landed, so its first fragments can be read
     // behind the last step's products.
-    Frags f0;
-    int buf, ahead;   // the current stage's buffer; stages started after it
+    struct Stream {
+        Frags f0;
+        int buf, ahead;   // the current stage's buffer; stages started after it
+    };
 
     template <typename N>
-    __device__ __forceinline__ void begin(N next) {
-        ahead = -1;
+    __device__ __forceinline__ void begin(Stream &st, N next) const {
+        int ahead = -1;
 #pragma unroll
         for (int s = 0; s < NS; ++s) ahead += next(s) ? 1 : 0;
-        landed<NS - 1>();
-        buf = 0;
-        read(f0, 0, 0);
+        landed<NS - 1>(ahead);
+        st.buf = 0;
+        st.ahead = ahead;
+        read(st.f0, 0, 0);
     }
 
     // Every wave's transfers of all but the last `F` stages started have landed, if all
     // those are under way (a wave's loads complete in order); else all of them.
     template <int F>
-    __device__ __forceinline__ void landed() const {
+    static __device__ __forceinline__ void landed(int ahead) {
         if (F > 0 && ahead == F)
             vm_wait<F *(MP + NP)>();
         else
@@ -232,23 +237,22 @@ struct Product {
     }
 
     template <typename N>
-    __device__ __forceinline__ void steps(int n, f16x (&acc)[MI][NI], N next) {
+    __device__ __forceinline__ void steps(Stream &st, int n, f16x (&acc)[MI][NI], N next) const {
         for (int t = 0; t < n; ++t) {
             Frags f1;
-            read(f1, buf, 1);
-            multiply(f0, acc);
+            read(f1, st.buf, 1);
+            multiply(st.f0, acc);
             interleave();
-            read(f0, buf, 2);
+            read(st.f0, st.buf, 2);
             multiply(f1, acc);
             interleave();
-            read(f1, buf, 3);
-            multiply(f0, acc);
+            read(f1, st.buf, 3);
+            multiply(st.f0, acc);
             interleave();
-            --ahead;   // from the next stage on
-            landed<NS - 2>();
-            ahead += next(buf) ? 1 : 0;
-            buf = NS == 2 ? buf ^ 1 : buf == NS - 1 ? 0 : buf + 1;
-            read(f0, buf, 0);
+            landed<NS - 2>(--st.ahead);   // counted from the next stage on
+            st.ahead += next(st.buf) ? 1 : 0;
+            st.buf = NS == 2 ? st.buf ^ 1 : st.buf == NS - 1 ? 0 : st.buf + 1;
+            read(st.f0, st.buf, 0);
             multiply(f1, acc);
             interleave();
         }
@@ -256,18 +260,18 @@ struct Product {
 
     // k from kbeg to kend, multiples of PK, of the operands as they are.  Leaves no
     // transfer in flight and every wave past its last read.
-    __device__ __forceinline__ void run(int kbeg, int kend, f16x (&acc)[MI][NI]) {
-        zero(acc);
-        if (kbeg >= kend) return;
+    __device__ __forceinline__ void run(int kbeg, int kend, f16x (&acc)[MI][NI]) const {
         int k = kbeg;
         auto next = [&](int b) FA2_INLINE {
-            if (k >= kend) return false;
-            issue(k, b);
+            const bool more = k < kend;
+            if (more) issue(k, b);
             k += PK;
-            return true;
+            return more;
         };
-        begin(next);
-        steps((kend - kbeg) / PK, acc, next);
+        Stream st;
+        begin(st, next);
+        zero(acc);
+        steps(st, (kend - kbeg) / PK, acc, next);
         lds_barrier();
     }
 };

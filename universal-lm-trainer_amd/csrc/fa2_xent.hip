@@ -183,11 +183,12 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
         }
         return true;
     };
-    pr.begin(next);
+    typename Pr::Stream stream;
+    pr.begin(stream, next);
     for (int t = t0; t < t1; ++t) {
         f16x acc[MI][NI];
         pr.zero(acc);
-        pr.steps(a.dp / PK, acc, next);
+        pr.steps(stream, a.dp / PK, acc, next);
         // Rows of this wave's part that are past the vocabulary (in the last tile) are left out.
         const int left = a.V - t * Pr::TM - pr.wm;
         auto add_tile = [&](auto tail, int j) FA2_INLINE {
@@ -402,13 +403,14 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
         }
         return true;
     };
-    pr.begin(next);
+    typename Pr::Stream stream;
+    pr.begin(stream, next);
     char *blk = out + (threadIdx.x >> 6) * 4096;
     for (int t = t0; t < t1; ++t) {
         const int v0 = a.p0 + t * Pr::TM;
         f16x acc[Pr::MI][Pr::NI];
         pr.zero(acc);
-        pr.steps(a.dp / PK, acc, next);
+        pr.steps(stream, a.dp / PK, acc, next);
 #pragma unroll
         for (int j = 0; j < Pr::NI; ++j) {
             T *o = static_cast<T *>(a.Pn) + (int64_t)(rb * Pr::TN + pr.wn + 32 * j) * a.piece + t * Pr::TM + pr.wm;

@@ -1,6 +1,7 @@
 """Minimal pre-norm decoder in the reference's shape, used to exercise the
 attention path inside a full training step (benchmark configuration 5) and in
-the model-level drop-in test.
+the model-level drop-in test; with ``fused=True`` it also runs what lies between
+two attention calls, and the loss, through the package's operators on token rows.
 
 It mirrors what reaches the attention kernel in the reference
 (reference @ None: train.py:1861-2105) -- fused QKV projection, q/k/v as
@@ -69,8 +70,12 @@ class Attention(nn.Module):
         (reference @ None: hf_template/modeling_universal_lm.py:228-251),
         through ``flash_attn_kvcache`` or, on the fallback path, SDPA with
         that mask spelled out."""
-        B, S, D = x.shape
-        q, k, v = (t.view(B, S, self.h, self.d).transpose(1, 2) for t in self.wqkv(x).chunk(3, dim=-1))
+        return self.cached(self.wqkv(x), cos, sin, cache)
+
+    def cached(self, qkv, cos, sin, cache):
+        """forward_cached from the fused QKV projection's output on."""
+        B, S, D = *qkv.shape[:2], qkv.shape[2] // 3
+        q, k, v = (t.view(B, S, self.h, self.d).transpose(1, 2) for t in qkv.chunk(3, dim=-1))
         fa = self.fa if self.use_kernel else None
         if fa is not None and fa.rope_can_use(q, k, cos, sin):
             q, k = fa.rope(q, k, cos, sin)
@@ -84,14 +89,31 @@ class Attention(nn.Module):
             attn = fa.flash_attn_kvcache(q, k, v, causal=True)
         else:
             Sk = k.shape[2]
-            mask = torch.ones(S, Sk, dtype=torch.bool, device=x.device).tril(Sk - S)
+            mask = torch.ones(S, Sk, dtype=torch.bool, device=qkv.device).tril(Sk - S)
             attn = F.scaled_dot_product_attention(q, k, v, attn_mask=mask)
         return self.wo(attn.transpose(1, 2).contiguous().view(B, S, D))
+
+
+class Proj8:
+    """A linear layer's weight in e4m3 with one scale an output, for rows that
+    ``rms_norm_fp8`` left in 8 bits; the product is the library's."""
+
+    def __init__(self, linear):
+        w = linear.weight.detach().float()
+        scale = (w.abs().amax(1, keepdim=True) / 448).clamp_min(2.0 ** -126)
+        self.w, self.scale = (w / scale).to(torch.float8_e4m3fn), scale.t().contiguous()
+
+    def __call__(self, q, scale, dtype):
+        y = torch._scaled_mm(q.reshape(-1, q.shape[-1]), self.w.t(), scale_a=scale.reshape(-1, 1), scale_b=self.scale,
+                             out_dtype=torch.bfloat16)   # the only output type of row-wise scales
+        return y.view(*q.shape[:-1], -1).to(dtype)
 
 
 class Block(nn.Module):
     def __init__(self, d_model, n_heads, d_ff, fa, use_kernel):
         super().__init__()
+        self.fa = fa
+        self.proj8 = None   # (wqkv, w1, w3) in 8 bits, for forward_cached_fused
         self.n1 = nn.RMSNorm(d_model, eps=1e-6)
         self.n2 = nn.RMSNorm(d_model, eps=1e-6)
         self.attn = Attention(d_model, n_heads, fa, use_kernel)
@@ -109,10 +131,51 @@ class Block(nn.Module):
         h = self.n2(x)
         return x + self.w2(F.silu(self.w1(h)) * self.w3(h))
 
+    def norm(self, n, branch, h, p):
+        """The last branch (None before the first block) added to the residual stream h
+        and the norm n of the sum: (y, h), y of the type the next linear layer takes."""
+        if branch is None:
+            dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else h.dtype
+            return self.fa.rms_norm(h, n.weight, eps=n.eps, out_dtype=dtype), h
+        return self.fa.add_rms_norm(branch, h, n.weight, eps=n.eps, dropout_p=p)
+
+    def forward_fused(self, branch, h, cos, sin, p):
+        """forward with the residual stream h and the branch that is still to be added
+        kept apart; returns the pair."""
+        y, h = self.norm(self.n1, branch, h, p)
+        y, h = self.norm(self.n2, self.attn(y, cos, sin), h, p)
+        return self.w2(F.silu(self.w1(y)) * self.w3(y)), h
+
+    def norm8(self, n, branch, h):
+        """norm in 8 bits, without dropout: (q, scale, h)."""
+        if branch is None:
+            return (*self.fa.rms_norm_fp8(h, n.weight, eps=n.eps), h)
+        return self.fa.rms_norm_fp8(branch, n.weight, eps=n.eps, residual=h)
+
+    def forward_cached_fused(self, branch, h, cos, sin, cache):
+        if self.proj8 is None:
+            y, h = self.norm(self.n1, branch, h, 0.0)
+            y, h = self.norm(self.n2, self.attn.forward_cached(y, cos, sin, cache), h, 0.0)
+            return self.w2(F.silu(self.w1(y)) * self.w3(y)), h
+        wqkv, w1, w3 = self.proj8
+        q, s, h = self.norm8(self.n1, branch, h)
+        a = self.attn.cached(wqkv(q, s, h.dtype), cos, sin, cache)
+        q, s, h = self.norm8(self.n2, a, h)
+        return self.w2(F.silu(w1(q, s, h.dtype)) * w3(q, s, h.dtype)), h
+
 
 class Decoder(nn.Module):
-    def __init__(self, vocab=32000, d_model=768, n_heads=12, n_layers=10, d_ff=2048, fa=None, use_kernel=True):
+    """``fused``: norms, residual additions, dropout and the loss through the package's
+    operators (GPU; the residual stream and its next branch are kept apart between
+    blocks).  ``dropout`` (with ``fused``): of the embedding and of every branch, in
+    training."""
+
+    def __init__(self, vocab=32000, d_model=768, n_heads=12, n_layers=10, d_ff=2048, fa=None, use_kernel=True,
+                 fused=False, dropout=0.0):
         super().__init__()
+        if fused and fa is None or dropout and not fused:
+            raise ValueError("fused needs the kernel module, and dropout needs fused")
+        self.fa, self.fused, self.dropout = fa, fused, dropout
         self.emb = nn.Embedding(vocab, d_model)
         self.layers = nn.ModuleList(Block(d_model, n_heads, d_ff, fa, use_kernel) for _ in range(n_layers))
         self.norm = nn.RMSNorm(d_model, eps=1e-6)
@@ -121,14 +184,33 @@ class Decoder(nn.Module):
         for p in self.parameters():  # std 0.02 init (train.py:2015-2022)
             nn.init.normal_(p, std=0.02) if p.dim() > 1 else nn.init.ones_(p)
 
-    def forward(self, ids):
+    def forward_hidden(self, ids):
+        """The final norm's output, which the tied head takes."""
         S = ids.shape[1]
         cos, sin = wl.rope_tables(S, d_model=self.d_model, head_dim=self.head_dim)
         cos, sin = cos.to(ids.device), sin.to(ids.device)
         x = self.emb(ids)
+        if self.fused:
+            p = self.dropout if self.training else 0.0
+            branch, h = None, self.fa.dropout(x, p)
+            for layer in self.layers:
+                branch, h = layer.forward_fused(branch, h, cos, sin, p)
+            return self.layers[-1].norm(self.norm, branch, h, p)[0]
         for layer in self.layers:
             x = layer(x, cos, sin)
-        return F.linear(self.norm(x), self.emb.weight)  # tied head
+        return self.norm(x)
+
+    def forward(self, ids):
+        return F.linear(self.forward_hidden(ids), self.emb.weight)  # tied head
+
+    def quantize(self):
+        """Projections behind a norm in 8 bits from now on, in cached (serving) calls of a
+        fused model."""
+        if not self.fused:
+            raise ValueError("8-bit projections need fused")
+        for layer in self.layers:
+            layer.proj8 = tuple(Proj8(m) for m in (layer.attn.wqkv, layer.w1, layer.w3))
+        return self
 
     def new_cache(self):
         return [[None, None] for _ in self.layers]
@@ -142,11 +224,18 @@ class Decoder(nn.Module):
         cos, sin = wl.rope_tables(max_len, d_model=self.d_model, head_dim=self.head_dim)
         cos, sin = (t[past:past + S].contiguous().to(ids.device) for t in (cos, sin))
         x = self.emb(ids)
+        if self.fused:
+            branch, h = None, x
+            for layer, c in zip(self.layers, cache):
+                branch, h = layer.forward_cached_fused(branch, h, cos, sin, c)
+            return F.linear(self.layers[-1].norm(self.norm, branch, h, 0.0)[0], self.emb.weight)
         for layer, c in zip(self.layers, cache):
             x = layer.forward_cached(x, cos, sin, c)
         return F.linear(self.norm(x), self.emb.weight)
 
     def loss(self, ids):
+        if self.fused:
+            return self.fa.linear_cross_entropy(self.forward_hidden(ids[:, :-1]), self.emb.weight, ids[:, 1:])
         logits = self.forward(ids[:, :-1])
         return F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), ids[:, 1:].reshape(-1))
 
