@@ -112,13 +112,13 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     p.strip = p.small ? 1 : (int)clamp(rt * nv / (4 * p.slots), 1, 4);
     // dx: sums for all token tiles, or, when those are few, for slices up to one item a slot.
     p.xcap = (int)(rt * nd > p.slots ? rt : clamp(p.slots / nd, 1, p.slots));
-    // dW: its k, the tokens, in slices no longer than a slot's share of a launch, and
-    // than a third of it in the last launch, which has no P to fill the slots with
-    // (stages of 64 k).
+    // dW: its k, the tokens, in slices (lengths in stages of 64 k).  Beside P, whose items
+    // fill the slots, none longer than a slot's share of the launch; without P, thirds of
+    // a share where a whole one is longer than half of it.
     const int64_t kt = rt * (tt / 64), both = nv * rt * (nd * 2 * (tt / 64)) / p.slots, fill = nv * rt * (p.dp / 64 + 4) / p.slots;
     auto slices = [&](int64_t len) { return (int)clamp((kt + len - 1) / (len > 4 ? len : 4), 1, p.pieces > 1 ? 4 : 16); };
-    p.wsplit = slices(both + fill);
-    p.wsplit_last = slices(both / 3);
+    p.wsplit = p.pieces > 1 ? slices(both + fill) : 1;
+    p.wsplit_last = kt > both / 2 ? slices(both / 3) : 1;
     const int wmax = p.wsplit > p.wsplit_last ? p.wsplit : p.wsplit_last;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += up256(bytes); return o; };

@@ -44,50 +44,68 @@ constexpr int PACK_ROWS = 64;   // packed rows a workgroup has at a time, at mos
 // whole tile of rows), and the tokens' packed rows.
 template <typename T>
 __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
-    __shared__ int wave_sum[16];
+    constexpr int Q = 16;                // targets a thread has at a time
+    __shared__ int before[16 * Q + 1];   // tokens that count in each run of 64 targets; then, before it
     __shared__ int src[PACK_ROWS];
     typedef typename vec_of<T>::v8 v8;
-    constexpr int Q = 16;   // targets a thread has at a time
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int share = ((int)a.rows + gridDim.x - 1) / gridDim.x;   // of the tokens' packed rows (at most 2^24 tokens)
-    const int64_t i0 = (int64_t)blockIdx.x * share, i1 = min(a.rows, i0 + share);
+    const int rows_n = (int)a.rows, i0 = blockIdx.x * share, i1 = min(rows_n, i0 + share);
     const bool vec = a.x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.d % 8 == 0;
     for (int j0 = blockIdx.x * a.pack_rows; j0 < a.rows_pad; j0 += gridDim.x * a.pack_rows) {
         int n = 0;   // tokens that count so far
-        for (int64_t r0 = 0; r0 < a.rows; r0 += 1024 * Q) {
-            const int64_t first = r0 + wave * (64 * Q) + lane;
+        for (int r0 = 0; r0 < rows_n; r0 += 1024 * Q) {
+            const int qs = min(Q, (rows_n - r0 + 1023) / 1024);   // in use
+            const int first = r0 + (int)threadIdx.x;              // run 16 q + wave: targets r0 + 1024 q + 64 wave ..
             int64_t t[Q];
             uint64_t m[Q];
-            int mine = 0;
 #pragma unroll
-            for (int q = 0; q < Q; ++q) t[q] = first + q * 64 < a.rows ? a.target[first + q * 64] : a.ignore;
+            for (int q = 0; q < Q; ++q)
+                if (q < qs) t[q] = first + q * 1024 < rows_n ? a.target[first + q * 1024] : a.ignore;
 #pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                m[q] = __ballot(first + q * 64 < a.rows && t[q] != a.ignore);
-                mine += __popcll(m[q]);
-            }
-            __syncthreads();   // the last round's sums have been read
-            if (lane == 0) wave_sum[wave] = mine;
-            __syncthreads();
-            int at = n;
-#pragma unroll
-            for (int w = 0; w < 16; ++w) {
-                at += w < wave ? wave_sum[w] : 0;
-                n += wave_sum[w];
-            }
-#pragma unroll
-            for (int q = 0; q < Q; ++q) {
-                const int64_t i = first + q * 64;
-                const bool in = m[q] >> lane & 1;
-                const int j = at + __popcll(m[q] & ((1ull << lane) - 1));
-                at += __popcll(m[q]);
-                if (i >= i0 && i < i1) a.pos[i] = in ? j : -1;
-                if (in && j >= j0 && j < j0 + a.pack_rows) {
-                    src[j - j0] = (int)i;
-                    a.rowmap[j] = (int)i;
-                    a.tgt[j] = t[q] >= 0 && t[q] < a.V ? (int)t[q] : -1;
+            for (int q = 0; q < Q; ++q)
+                if (q < qs) {
+                    m[q] = __ballot(first + q * 1024 < rows_n && t[q] != a.ignore);
+                    if (lane == 0) before[16 * q + wave] = __popcll(m[q]);
                 }
+            __syncthreads();
+            if (wave == 0) {   // exclusive sums over the runs, four a lane
+                int c[4], sum = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    c[k] = 4 * lane + k < 16 * qs ? before[4 * lane + k] : 0;
+                    sum += c[k];
+                }
+                int up = sum;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int v = __shfl_up(up, o);
+                    up += lane >= o ? v : 0;
+                }
+                int at = n + up - sum;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    before[4 * lane + k] = at;
+                    at += c[k];
+                }
+                if (lane == 63) before[16 * Q] = at;
             }
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                if (q < qs) {
+                    const int i = first + q * 1024;
+                    const bool in = m[q] >> lane & 1;
+                    const int j = before[16 * q + wave] + __popcll(m[q] & ((1ull << lane) - 1));
+                    if (i >= i0 && i < i1) a.pos[i] = in ? j : -1;
+                    if (in && j >= j0 && j < j0 + a.pack_rows) {
+                        src[j - j0] = i;
+                        a.rowmap[j] = i;
+                        a.tgt[j] = t[q] >= 0 && t[q] < a.V ? (int)t[q] : -1;
+                    }
+                }
+            n = before[16 * Q];
+            __syncthreads();   // before is free
         }
         if (j0 == 0 && threadIdx.x == 0) {
             a.count[N_TOKENS] = n;
@@ -563,21 +581,33 @@ __global__ __launch_bounds__(256) void xent_dw_join_kernel(const XentArgs a) {
 }
 
 // dx of every token: the slices' sums, rounded once; zeros where a token does not
-// count.  One wave a token.
+// count.  Four columns a thread, eight slices' loads at a time (one wave a token, slice
+// after slice: 38 us for 43 slices of 188 tokens).
 template <typename T, int MP>
 __global__ __launch_bounds__(256) void xent_dx_out_kernel(const XentArgs a) {
-    const int n = a.count[N_TOKENS], lane = threadIdx.x & 63;
+    const int n = a.count[N_TOKENS];
     const XentWork k = xent_work<MP>(a, n);
     const float u = xent_unscale(a, n);
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.rows; i += (int64_t)gridDim.x * 4) {
-        const int j = a.pos[i];
-        for (int c = lane * 8; c < a.d; c += 512) {
-            f8 x = {};
-            if (j >= 0)
-                for (int s = 0; s < k.xs; ++s)
-                    x += *reinterpret_cast<const f8 *>(a.acc + ((int64_t)s * k.rt * (64 * MP) + j) * a.dp + c);
-            store8<T>(static_cast<T *>(a.dx) + i * a.d, c, a.d, a.d % 8 == 0, x * u);
+    const uint32_t per = (a.d + 3) / 4;
+    const uint64_t total = (uint64_t)a.rows * per;
+    const int64_t slice = (int64_t)k.rt * (64 * MP) * a.dp;
+    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
+        const uint32_t i = total < 1u << 31 ? (uint32_t)e / per : (uint32_t)(e / per);   // at most 2^24 tokens
+        const int c = (int)(e - (uint64_t)i * per) * 4, j = a.pos[i];
+        f4 x = {0.f, 0.f, 0.f, 0.f};
+        if (j >= 0) {
+            const float *p = a.acc + (int64_t)j * a.dp + c;
+            int s = 0;
+            for (; s + 8 <= k.xs; s += 8) {
+                f4 v[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] = *reinterpret_cast<const f4 *>(p + (s + q) * slice);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) x += v[q];
+            }
+            for (; s < k.xs; ++s) x += *reinterpret_cast<const f4 *>(p + s * slice);
         }
+        store4(static_cast<T *>(a.dx) + (int64_t)i * a.d, c, a.d, a.d % 4 == 0, x * u);
     }
 }
 
@@ -644,7 +674,7 @@ hipError_t launch_xent_grad(const XentArgs &a, hipStream_t st) {
 }
 
 hipError_t launch_xent_bwd_finish(const XentArgs &a, hipStream_t st) {
-    const unsigned grid = at_most((a.rows + 3) / 4, 8192);
+    const unsigned grid = at_most((a.rows * ((a.d + 3) / 4) + 255) / 256, 16384);
     if (a.type == FA2_F16) {
         if (a.small)
             FA2_LAUNCH((xent_dx_out_kernel<_Float16, 2>), grid, 256);
