@@ -65,6 +65,12 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(const NormF
         f4 h[NCH], w[NCH];
 #pragma unroll
         for (int c = 0; c < NCH; ++c) h[c] = load4(x, (c * G + t) * 4, a.cols, vec);
+        // 8 bits: mostly few rows, where the weights' latency counts.  (Loaded here for the others too, 138 -> 141 us forward
+        // and backward at 32768 x 768.)
+        if (FP8) {
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) w[c] = load4_typed(a.w, a.w_type, (c * G + t) * 4, a.cols, vec);
+        }
         if (a.drop_thr) {
             const uint32_t part = a.seed_part ^ dropout_row_term((int)row);
 #pragma unroll
@@ -87,8 +93,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(const NormF
                 h[c] = __builtin_convertvector(__builtin_convertvector(h[c], typename vec_of<TR>::v4), f4);
             }
         }
+        if (!FP8) {
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) w[c] = load4_typed(a.w, a.w_type, (c * G + t) * 4, a.cols, vec);
+            for (int c = 0; c < NCH; ++c) w[c] = load4_typed(a.w, a.w_type, (c * G + t) * 4, a.cols, vec);
+        }
         float ss = 0.f;
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
@@ -113,9 +121,12 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void norm_fwd_kernel(const NormF
             float scale = amax / FP8_MAX;
             scale = scale < FP8_MIN_SCALE ? FP8_MIN_SCALE : scale;
             if (t == 0) a.scale[row] = scale;
+            // A product by the reciprocal: within 2^-23 of the quotient, which moves a value only where it lies that
+            // near the middle of two e4m3 steps.
+            const float inv = 1.f / scale;
             uint8_t *y = static_cast<uint8_t *>(a.y) + row * a.cols;
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) store_fp8(y, (c * G + t) * 4, a.cols, vec, h[c] / scale);
+            for (int c = 0; c < NCH; ++c) store_fp8(y, (c * G + t) * 4, a.cols, vec, h[c] * inv);
         } else {
             TY *y = static_cast<TY *>(a.y) + row * a.cols;
 #pragma unroll

@@ -142,7 +142,6 @@ struct XentArgs {
     const void *P;                 // [rows_pad, piece]
     int p0, p1;                    // the piece whose P is formed, into Pn
     void *Pn;
-    int strip;                     // tiles of P an item
     int xcap;                      // dx: token tiles there are sums for, in all slices
     float *acc;                    // [xcap tiles, dp]
     int wsplit;                    // dW: slices of the tokens

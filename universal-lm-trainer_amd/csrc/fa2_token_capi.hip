@@ -69,7 +69,7 @@ struct XentPlan {
     int rows_pad, dp;
     bool small;
     int stat_tile_n, stat_tile_m, stat_slots, stat_rounds, stat_items;
-    int slots, piece, pieces, strip, xcap;
+    int slots, piece, pieces, xcap;
     int wsplit, wsplit_last;
     // offsets in the state
     size_t count, lse, tgt, rowmap, pos, xc, state_bytes;
@@ -109,7 +109,6 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     p.small = (R / 256) * (p.piece / 256) < 256;
     p.slots = p.small ? 512 : 256;
     const int64_t tt = p.small ? 128 : 256, rt = R / tt, nd = (d + tt - 1) / tt, nv = p.piece / tt;
-    p.strip = p.small ? 1 : (int)clamp(rt * nv / (4 * p.slots), 1, 4);
     // dx: sums for all token tiles, or, when those are few, for slices up to one item a slot.
     p.xcap = (int)(rt * nd > p.slots ? rt : clamp(p.slots / nd, 1, p.slots));
     // dW: its k, the tokens, in slices (lengths in stages of 64 k).  Beside P, whose items
@@ -213,7 +212,6 @@ fa2::XentArgs xent_args(const fa2_xent_params *p, const XentPlan &pl, char *s) {
     a.slots = pl.slots;
     a.piece = pl.piece;
     a.pieces = pl.pieces;
-    a.strip = pl.strip;
     a.xcap = pl.xcap;
     return a;
 }

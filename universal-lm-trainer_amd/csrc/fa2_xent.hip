@@ -113,22 +113,30 @@ __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
         }
         if ((int)threadIdx.x < a.pack_rows && j0 + (int)threadIdx.x >= n) a.tgt[j0 + threadIdx.x] = -1;
         __syncthreads();
-        // Pieces of 8 elements, a thread's next to those of its neighbours.
-        const int rows = min(a.pack_rows, (n + XENT_PAD - 1) / XENT_PAD * XENT_PAD - j0), per = a.dp / 8;
-        for (int p = threadIdx.x; p < rows * per; p += 1024) {
-            const int r = p / per, c = (p - r * per) * 8;
-            v8 v = {};
-            if (j0 + r < n) {
-                const T *x = static_cast<const T *>(a.x) + (int64_t)src[r] * a.x_stride;
-                if (vec) {
-                    if (c < a.d) v = *reinterpret_cast<const v8 *>(x + c);
-                } else {
+        // Wave w: rows w, w + 16, .., up to four at a time; 8 elements a lane.
+        const int rows = min(a.pack_rows, (n + XENT_PAD - 1) / XENT_PAD * XENT_PAD - j0);
+        for (int c = lane * 8; c < a.dp; c += 512) {
+            v8 v[PACK_ROWS / 16];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (c + e < a.d) v[e] = x[c + e];
+            for (int q = 0; q < PACK_ROWS / 16; ++q) {
+                const int r = wave + 16 * q;
+                v[q] = v8{};
+                if (r < rows && j0 + r < n) {
+                    const T *x = static_cast<const T *>(a.x) + (int64_t)src[r] * a.x_stride;
+                    if (vec) {
+                        if (c < a.d) v[q] = *reinterpret_cast<const v8 *>(x + c);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (c + e < a.d) v[q][e] = x[c + e];
+                    }
                 }
             }
-            *reinterpret_cast<v8 *>(static_cast<T *>(a.xc) + (int64_t)(j0 + r) * a.dp + c) = v;
+#pragma unroll
+            for (int q = 0; q < PACK_ROWS / 16; ++q) {
+                const int r = wave + 16 * q;
+                if (r < rows) *reinterpret_cast<v8 *>(static_cast<T *>(a.xc) + (int64_t)(j0 + r) * a.dp + c) = v[q];
+            }
         }
         __syncthreads();   // src is free
     }
@@ -365,8 +373,10 @@ struct XentWork {
     int rt;            // tiles of tokens that count
     int dw, dx, p;     // items
     int xs;            // slices of dx's k
+    int strip;         // tiles of P an item
 };
 
+constexpr int P_ROUNDS = 4;      // items of P a slot, at most
 constexpr int P_TILE_EXTRA = 4;  // stages that the softmax of a tile of P takes as long as
 
 template <int MP>
@@ -382,19 +392,36 @@ __device__ __forceinline__ XentWork xent_work(const XentArgs &a, int n) {
     k.xs = max(1, min((a.piece / PK + share - 1) / share, a.xcap / max(k.rt, 1)));
     k.dw = a.dw ? nd * nv * a.wsplit : 0;
     k.dx = a.dx && nv > 0 ? nd * k.rt * k.xs : 0;
-    k.p = k.rt * ((nvp + a.strip - 1) / a.strip);
+    // P: tiles of one token tile in strips, whose stages are one stream (MP = 2: single
+    // tiles, since their output goes through the panels).  Alone, in the rounds of equal
+    // strips that take the fewest tiles one after the other; beside the others short
+    // ones, up to four a slot.
+    const int tiles = k.rt * nvp;
+    k.strip = MP == 2 ? 1 : max(1, (tiles + P_ROUNDS * a.slots - 1) / (P_ROUNDS * a.slots));
+    if (MP == 4 && k.dw + k.dx == 0) {
+        int cost = INT32_MAX;
+        for (int r = 1; r <= P_ROUNDS; ++r) {
+            const int s = max(1, (tiles + r * a.slots - 1) / (r * a.slots));
+            const int c = (k.rt * ((nvp + s - 1) / s) + a.slots - 1) / a.slots * (4 * s + 1);   // a strip's start: a quarter tile
+            if (c < cost) {
+                cost = c;
+                k.strip = s;
+            }
+        }
+    }
+    k.p = k.rt * ((nvp + k.strip - 1) / k.strip);
     return k;
 }
 
-// a.strip tiles of P: logits again, softmax, minus one at the target; M side
+// k.strip tiles of P: logits again, softmax, minus one at the target; M side
 // vocabulary rows, N side tokens.  In units of 1 / P_SCALE, times the row's factor.
 template <typename T, int MP>
 __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k, int item, int n, char *mem, char *out) {
     typedef Product<T, true, true, false, true, MP, MP, 2, 4> Pr;
-    const int tiles = (a.p1 - a.p0 + Pr::TM - 1) / Pr::TM, strips = (tiles + a.strip - 1) / a.strip;
+    const int tiles = (a.p1 - a.p0 + Pr::TM - 1) / Pr::TM, strips = (tiles + k.strip - 1) / k.strip;
     // groups of 8 token tiles, in a group the tokens fastest
     const int g = item / (8 * strips), gs = min(8, k.rt - 8 * g), in = item - g * 8 * strips;
-    const int rb = 8 * g + in % gs, t0 = in / gs * a.strip, t1 = min(tiles, t0 + a.strip);
+    const int rb = 8 * g + in % gs, t0 = in / gs * k.strip, t1 = min(tiles, t0 + k.strip);
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
     Pr pr;
     pr.init(mem);
@@ -581,19 +608,18 @@ __global__ __launch_bounds__(256) void xent_dw_join_kernel(const XentArgs a) {
 }
 
 // dx of every token: the slices' sums, rounded once; zeros where a token does not
-// count.  Four columns a thread, eight slices' loads at a time (one wave a token, slice
-// after slice: 38 us for 43 slices of 188 tokens).
+// count.  One wave 256 columns of a token, eight slices' loads at a time (whole rows a
+// wave, slice after slice: 38 us for 43 slices of 188 tokens).
 template <typename T, int MP>
 __global__ __launch_bounds__(256) void xent_dx_out_kernel(const XentArgs a) {
     const int n = a.count[N_TOKENS];
     const XentWork k = xent_work<MP>(a, n);
     const float u = xent_unscale(a, n);
-    const uint32_t per = (a.d + 3) / 4;
-    const uint64_t total = (uint64_t)a.rows * per;
     const int64_t slice = (int64_t)k.rt * (64 * MP) * a.dp;
-    for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (uint64_t)gridDim.x * 256) {
-        const uint32_t i = total < 1u << 31 ? (uint32_t)e / per : (uint32_t)(e / per);   // at most 2^24 tokens
-        const int c = (int)(e - (uint64_t)i * per) * 4, j = a.pos[i];
+    const int c = blockIdx.y * 256 + (threadIdx.x & 63) * 4;
+    if (c >= a.d) return;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.rows; i += (int64_t)gridDim.x * 4) {
+        const int j = a.pos[i];
         f4 x = {0.f, 0.f, 0.f, 0.f};
         if (j >= 0) {
             const float *p = a.acc + (int64_t)j * a.dp + c;
@@ -607,7 +633,7 @@ __global__ __launch_bounds__(256) void xent_dx_out_kernel(const XentArgs a) {
             }
             for (; s < k.xs; ++s) x += *reinterpret_cast<const f4 *>(p + s * slice);
         }
-        store4(static_cast<T *>(a.dx) + (int64_t)i * a.d, c, a.d, a.d % 4 == 0, x * u);
+        store4(static_cast<T *>(a.dx) + i * a.d, c, a.d, a.d % 4 == 0, x * u);
     }
 }
 
@@ -640,7 +666,8 @@ hipError_t grad(const XentArgs &a, hipStream_t st) {
     constexpr int TT = 64 * MP;
     const int rt = a.rows_pad / TT, nd = (a.d + TT - 1) / TT, nv = (a.v1 - a.v0 + TT - 1) / TT, np = (a.p1 - a.p0 + TT - 1) / TT;
     // the most items there can be
-    const int items = (a.dw ? nd * nv * a.wsplit : 0) + (a.dx && nv ? nd * a.xcap : 0) + rt * ((np + a.strip - 1) / a.strip);
+    const int strips = MP == 2 || rt * np < P_ROUNDS * a.slots + rt ? rt * np : P_ROUNDS * a.slots + rt;
+    const int items = (a.dw ? nd * nv * a.wsplit : 0) + (a.dx && nv ? nd * a.xcap : 0) + strips;
     if (items > 0) FA2_LAUNCH((xent_grad_kernel<T, MP>), items, 512);
     if (nv && a.dw && a.wsplit > 1) FA2_LAUNCH(xent_dw_join_kernel<T>, at_most((a.v1 - a.v0 + 3) / 4, 8192), 256);
     return hipSuccess;
@@ -674,7 +701,7 @@ hipError_t launch_xent_grad(const XentArgs &a, hipStream_t st) {
 }
 
 hipError_t launch_xent_bwd_finish(const XentArgs &a, hipStream_t st) {
-    const unsigned grid = at_most((a.rows * ((a.d + 3) / 4) + 255) / 256, 16384);
+    const dim3 grid(at_most((a.rows + 3) / 4, 4096), (a.d + 255) / 256);
     if (a.type == FA2_F16) {
         if (a.small)
             FA2_LAUNCH((xent_dx_out_kernel<_Float16, 2>), grid, 256);
