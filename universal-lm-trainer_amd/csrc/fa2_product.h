@@ -201,7 +201,7 @@ struct Product {
     }
 
     // A stream of stages.  begin() starts the first NS and reads the first
-    // fragments; steps() consumes n stages.  next(buf) starts the following stage's
+    // fragments; steps() consumes n stages (at least one) into a tile's accumulators.  next(buf) starts the following stage's
     // transfers into buffer buf and returns whether there was one left.
     //
     // The fragments of each k step are read while the step before is multiplied.
@@ -236,26 +236,33 @@ struct Product {
         lds_barrier();
     }
 
+    // FIRST: the accumulators start from zero, as the constant operand of their first
+    // products (cleared registers cost 2% at K = 768).
+    template <bool FIRST, typename N>
+    __device__ __forceinline__ void step(Stream &st, f16x (&acc)[MI][NI], N &next) const {
+        Frags f1;
+        read(f1, st.buf, 1);
+        if (FIRST) zero(acc);
+        multiply(st.f0, acc);
+        interleave();
+        read(st.f0, st.buf, 2);
+        multiply(f1, acc);
+        interleave();
+        read(f1, st.buf, 3);
+        multiply(st.f0, acc);
+        interleave();
+        landed<NS - 2>(--st.ahead);   // counted from the next stage on
+        st.ahead += next(st.buf) ? 1 : 0;
+        st.buf = NS == 2 ? st.buf ^ 1 : st.buf == NS - 1 ? 0 : st.buf + 1;
+        read(st.f0, st.buf, 0);
+        multiply(f1, acc);
+        interleave();
+    }
+
     template <typename N>
     __device__ __forceinline__ void steps(Stream &st, int n, f16x (&acc)[MI][NI], N next) const {
-        for (int t = 0; t < n; ++t) {
-            Frags f1;
-            read(f1, st.buf, 1);
-            multiply(st.f0, acc);
-            interleave();
-            read(st.f0, st.buf, 2);
-            multiply(f1, acc);
-            interleave();
-            read(f1, st.buf, 3);
-            multiply(st.f0, acc);
-            interleave();
-            landed<NS - 2>(--st.ahead);   // counted from the next stage on
-            st.ahead += next(st.buf) ? 1 : 0;
-            st.buf = NS == 2 ? st.buf ^ 1 : st.buf == NS - 1 ? 0 : st.buf + 1;
-            read(st.f0, st.buf, 0);
-            multiply(f1, acc);
-            interleave();
-        }
+        step<true>(st, acc, next);
+        for (int t = 1; t < n; ++t) step<false>(st, acc, next);
     }
 
     // k from kbeg to kend, multiples of PK, of the operands as they are.  Leaves no
@@ -270,11 +277,17 @@ struct Product {
         };
         Stream st;
         begin(st, next);
-        zero(acc);
-        steps(st, (kend - kbeg) / PK, acc, next);
+        if (kbeg < kend)
+            steps(st, (kend - kbeg) / PK, acc, next);
+        else
+            zero(acc);
         lds_barrier();
     }
 };
+
+// Swizzle of store_rows: 16 consecutive rows' 8-byte writes of one column group, and two
+// rows' 16-byte reads, touch distinct banks.
+__device__ __forceinline__ int swz_out(int r) { return (r ^ (r >> 3)) & 7; }
 
 // store_rows_f16 for either 16-bit type: a wave's 32 x 64 block in two
 // accumulators (acc0: columns 0..31, acc1: 32..63, row = lane & 31), times mul, as
@@ -293,13 +306,13 @@ __device__ __forceinline__ void store_rows(const f16x &acc0, const f16x &acc1, f
             f4 x;
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[j] = (db ? acc1 : acc0)[4 * i + j] * mul;
-            *reinterpret_cast<v4 *>(blk + c * 128 + (((4 * db + i) ^ (c & 7)) << 4) + 8 * g2) = __builtin_convertvector(x, v4);
+            *reinterpret_cast<v4 *>(blk + c * 128 + (((4 * db + i) ^ swz_out(c)) << 4) + 8 * g2) = __builtin_convertvector(x, v4);
         }
     const int ch = lane & 7;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int r = 8 * k + (lane >> 3);
-        const v8 v = *reinterpret_cast<const v8 *>(blk + r * 128 + ((ch ^ (r & 7)) << 4));
+        const v8 v = *reinterpret_cast<const v8 *>(blk + r * 128 + ((ch ^ swz_out(r)) << 4));
         if (r < nrows) {
             T *p = dst + r * stride + 8 * ch;
             if (vec16 && 8 * ch + 8 <= ncols) {

@@ -213,7 +213,6 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
     pr.begin(stream, next);
     for (int t = t0; t < t1; ++t) {
         f16x acc[MI][NI];
-        pr.zero(acc);
         pr.steps(stream, a.dp / PK, acc, next);
         // Rows of this wave's part that are past the vocabulary (in the last tile) are left out.
         const int left = a.V - t * Pr::TM - pr.wm;
@@ -454,7 +453,6 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
     for (int t = t0; t < t1; ++t) {
         const int v0 = a.p0 + t * Pr::TM;
         f16x acc[Pr::MI][Pr::NI];
-        pr.zero(acc);
         pr.steps(stream, a.dp / PK, acc, next);
 #pragma unroll
         for (int j = 0; j < Pr::NI; ++j) {
