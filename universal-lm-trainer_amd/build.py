@@ -27,8 +27,8 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
-HIP_SOURCES = ["fa2_fwd.hip", "fa2_bwd.hip", "fa2_rope.hip", "fa2_norm.hip", "fa2_dropout.hip", "fa2_xent.hip",
-               "fa2_capi.hip", "fa2_token_capi.hip"]
+HIP_SOURCES = ["fa2_fwd.hip", "fa2_bwd.hip", "fa2_rope.hip", "fa2_norm.hip", "fa2_norm_bwd.hip",
+               "fa2_xent.hip", "fa2_dropout.hip", "fa2_capi.hip", "fa2_token_capi.hip"]
 LIB_NAME = "libfa2_mi355x.so"
 EXT_NAME = "_fa2_torch"
 

@@ -256,6 +256,7 @@ int fa2_rms_norm_fwd(const fa2_rms_norm_params *p, void *stream) {
     a.seed_part = seed_part(p->seed);
     a.drop_thr = fa2_dropout_threshold(p->dropout_p);
     a.inv_keep = inv_keep(p->dropout_p);
+    a.stream = fa2::rows_stream(p->rows * p->cols * (int64_t)(type_size(p->x_type) + (p->residual ? type_size(rtype) : 0)));
     return launched("rms_norm", fa2::launch_norm_fwd(a, p->x_type, rtype, p->y_type, (hipStream_t)stream));
 }
 
@@ -302,6 +303,7 @@ int fa2_rms_norm_bwd(const fa2_rms_norm_bwd_params *p, void *workspace, size_t w
     a.seed_part = seed_part(p->seed);
     a.drop_thr = fa2_dropout_threshold(p->dropout_p);
     a.inv_keep = inv_keep(p->dropout_p);
+    a.stream = fa2::rows_stream(p->rows * p->cols * (int64_t)(type_size(p->y_type) + type_size(p->h_type) * (p->dh ? 2 : 1)));
     return launched("rms_norm backward", fa2::launch_norm_bwd(a, p->x_type, p->h_type, p->y_type, (hipStream_t)stream));
 }
 
