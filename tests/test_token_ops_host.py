@@ -150,3 +150,67 @@ def test_cpu_tensors_are_refused():
                  lambda: fa.dropout(x, 0.1), lambda: fa.linear_cross_entropy(x.half(), torch.zeros(5, 8).half(), t)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_plans_stay_inside_their_buffers(tmp_path):
+    """The slices that the kernels choose from the number of tokens that count fit the grids and buffers that the host sized
+    without knowing it, over many sizes: forward slices, dx slices, items of every backward launch."""
+    import os
+    import subprocess
+    csrc = os.path.join(capi.PKG, "csrc")
+    src = tmp_path / "plans.cpp"
+    src.write_text('#include "%s/fa2_token_capi.hip"\n' % csrc + r"""
+#include <cstdio>
+#include <cstdlib>
+using namespace fa2;
+template <int MP> static int check(XentArgs a, int n) {
+    constexpr int TT = 64 * MP;
+    const XentWork k = xent_work<MP>(a, n);
+    const int nvp = (a.p1 - a.p0 + TT - 1) / TT;
+    if (k.rt != (n + TT - 1) / TT || k.xs < 1 || k.strip < 1) return 1;
+    if ((int64_t)k.xs * k.rt > a.xcap) return 2;
+    if ((int64_t)k.dw + k.dx + k.p > xent_work_most<MP>(a)) return 3;
+    if (MP == 2 && k.strip != 1) return 4;
+    if ((int64_t)k.p * k.strip < (int64_t)k.rt * nvp) return 5;
+    if (k.rt * TT > a.rows_pad) return 6;
+    return 0;
+}
+int main() {
+    srand(1);
+    auto lo = [](double most) { double u = rand() / (RAND_MAX + 1.0); return (int64_t)exp(u * log(most)); };
+    for (int it = 0; it < 200000; ++it) {
+        const int64_t rows = lo(it % 3 ? 40000 : 16777217);
+        const int d = (int)lo(8193), V = (int)lo(it % 5 ? 300000 : 16777217);
+        const XentPlan p = xent_plan(rows, d, V);
+        fa2_xent_params q;
+        memset(&q, 0, sizeof(q));
+        q.rows = rows; q.hidden = d; q.vocab = V;
+        XentArgs a = xent_args(&q, p, nullptr);
+        a.dw = a.dx = (void *)16;
+        const int n = (int)(it % 4 == 0 ? rows : lo((double)rows + 1) - (it % 7 == 0));
+        const int s = xent_stat_splits(a.stat_tile_n, a.stat_tile_m, a.stat_slots, a.stat_rounds, n, V);
+        const int rt = n > 0 ? (n + a.stat_tile_n - 1) / a.stat_tile_n : 0;
+        int bad = 0;
+        if (s < 1 || (int64_t)rt * s > a.stat_items) bad = 10;
+        if (s > (V + a.stat_tile_m - 1) / a.stat_tile_m) bad = 11;
+        if (a.stat_items > (1 << 22)) bad = 12;                       // 2^22 workgroups of 512 threads
+        for (int i = 0; i <= a.pieces && !bad; ++i) {
+            auto edge = [&](int k) { return (int64_t)k * a.piece < V ? k * a.piece : V; };
+            a.v0 = i ? edge(i - 1) : 0; a.v1 = i ? edge(i) : 0; a.p0 = edge(i); a.p1 = edge(i + 1);
+            a.wsplit = i == a.pieces ? p.wsplit_last : p.wsplit;
+            if (a.wsplit < 1 || a.wsplit > 16 || (i && a.v1 <= a.v0)) bad = 13;
+            if (!bad) bad = a.small ? check<2>(a, n) : check<4>(a, n);
+            if (i > 3 && i < a.pieces - 2) i = a.pieces - 3;
+        }
+        if (a.piece % 256 || (int64_t)a.pieces * a.piece < V || a.piece >= 1 << 23) bad = 14;
+        if (bad) { printf("%d: rows %lld d %d V %d n %d\n", bad, (long long)rows, d, V, n); return 1; }
+    }
+    puts("fits");
+}
+""")
+    hipcc = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "bin", "hipcc")
+    lib = os.path.dirname(capi.LIB)
+    subprocess.run([hipcc, "-x", "hip", "--offload-host-only", "-O2", "-std=c++17", str(src), "-o", str(tmp_path / "plans"),
+                    f"-L{lib}", "-lfa2_mi355x", f"-Wl,-rpath,{lib}"], check=True, capture_output=True)
+    out = subprocess.run([str(tmp_path / "plans")], capture_output=True, text=True)
+    assert out.returncode == 0 and "fits" in out.stdout, out.stdout

@@ -153,6 +153,72 @@ struct XentArgs {
     void *dx, *dw;                 // [N, d], [V, d]; null: not wanted
 };
 
+// The work of one launch of the backward: dW and dx of a piece, and P of the piece
+// after it, as items of one grid, the long ones first; P's many short items fill the
+// compute units that the others leave.  Lengths are in stages of 64 k; tiles are
+// 64 MP on a side.
+struct XentWork {
+    int rt;            // tiles of tokens that count
+    int dw, dx, p;     // items
+    int xs;            // slices of dx's k
+    int strip;         // tiles of P an item
+};
+
+constexpr int P_ROUNDS = 4;         // items of P a slot, at most
+constexpr int P_TILE_EXTRA = 4;     // stages that the softmax of a tile of P takes as long as
+
+template <typename N>
+__host__ __device__ inline N larger(N a, N b) {
+    return a > b ? a : b;
+}
+template <typename N>
+__host__ __device__ inline N smaller(N a, N b) {
+    return a < b ? a : b;
+}
+
+template <int MP>
+__host__ __device__ inline XentWork xent_work(const XentArgs &a, int n) {
+    constexpr int TT = 64 * MP;
+    XentWork k;
+    const int nd = (a.d + TT - 1) / TT, nv = (a.v1 - a.v0 + TT - 1) / TT, nvp = (a.p1 - a.p0 + TT - 1) / TT;
+    k.rt = (n + TT - 1) / TT;
+    // Slices of dx: no longer than three quarters of a slot's share of a launch (with
+    // pieces of full width; the same number for every piece).
+    const int64_t total = (int64_t)(a.piece / TT) * k.rt * (nd * 2 * MP + (a.pieces > 1 ? a.dp / XENT_KPAD + P_TILE_EXTRA : 0));
+    const int share = (int)larger((int64_t)4, total * 3 / (4 * a.slots));
+    k.xs = larger(1, smaller((a.piece / XENT_KPAD + share - 1) / share, a.xcap / larger(k.rt, 1)));
+    k.dw = a.dw ? nd * nv * a.wsplit : 0;
+    k.dx = a.dx && nv > 0 ? nd * k.rt * k.xs : 0;
+    // P: tiles of one token tile in strips, whose stages are one stream (MP = 2: single
+    // tiles, since their output goes through the panels).  Alone, in the rounds of equal
+    // strips that take the fewest tiles one after the other; beside the others short
+    // ones, up to four a slot.
+    const int tiles = k.rt * nvp;
+    k.strip = MP == 2 ? 1 : larger(1, (tiles + P_ROUNDS * a.slots - 1) / (P_ROUNDS * a.slots));
+    if (MP == 4 && k.dw + k.dx == 0) {
+        int cost = INT32_MAX;
+        for (int r = 1; r <= P_ROUNDS; ++r) {
+            const int s = larger(1, (tiles + r * a.slots - 1) / (r * a.slots));
+            const int c = (k.rt * ((nvp + s - 1) / s) + a.slots - 1) / a.slots * (4 * s + 1);   // a strip's start: a quarter tile
+            if (c < cost) {
+                cost = c;
+                k.strip = s;
+            }
+        }
+    }
+    k.p = k.rt * ((nvp + k.strip - 1) / k.strip);
+    return k;
+}
+
+// The most items that xent_work can give, whatever number of tokens counts.
+template <int MP>
+inline int xent_work_most(const XentArgs &a) {
+    constexpr int TT = 64 * MP;
+    const int rt = a.rows_pad / TT, nd = (a.d + TT - 1) / TT, nv = (a.v1 - a.v0 + TT - 1) / TT, np = (a.p1 - a.p0 + TT - 1) / TT;
+    const int strips = MP == 2 ? rt * np : smaller(rt * np, P_ROUNDS * a.slots + rt);
+    return (a.dw ? nd * nv * a.wsplit : 0) + (a.dx && nv ? nd * a.xcap : 0) + strips;
+}
+
 hipError_t launch_xent_fwd(const XentArgs &a, hipStream_t st);
 hipError_t launch_xent_pad_weight(const void *w, int64_t w_stride, void *out, int V, int d, int dp, int type, hipStream_t st);
 hipError_t launch_xent_bwd_prepare(const XentArgs &a, hipStream_t st);

@@ -21,8 +21,6 @@
 // the matrix units; the gradients themselves are rounded to the same type.  P is
 // scaled so that its largest possible value is 2^15: in fp16 probabilities down
 // to 2^-29 stay normal numbers.
-#include <type_traits>
-
 #include "fa2_product.h"
 
 namespace fa2 {
@@ -364,54 +362,6 @@ __device__ __forceinline__ float xent_unscale(const XentArgs &a, int n) {
     return (a.reduction == FA2_REDUCE_MEAN ? a.g[0] / (float)n : a.g[0]) / P_SCALE;
 }
 
-// The work of one launch of the backward: dW and dx of a piece, and P of the piece
-// after it, as items of one grid, the long ones first; P's many short items fill the
-// compute units that the others leave.  Lengths are in stages of 64 k; tiles are
-// 64 MP on a side.
-struct XentWork {
-    int rt;            // tiles of tokens that count
-    int dw, dx, p;     // items
-    int xs;            // slices of dx's k
-    int strip;         // tiles of P an item
-};
-
-constexpr int P_ROUNDS = 4;      // items of P a slot, at most
-constexpr int P_TILE_EXTRA = 4;  // stages that the softmax of a tile of P takes as long as
-
-template <int MP>
-__device__ __forceinline__ XentWork xent_work(const XentArgs &a, int n) {
-    constexpr int TT = 64 * MP;
-    XentWork k;
-    const int nd = (a.d + TT - 1) / TT, nv = (a.v1 - a.v0 + TT - 1) / TT, nvp = (a.p1 - a.p0 + TT - 1) / TT;
-    k.rt = (n + TT - 1) / TT;
-    // Slices of dx: no longer than three quarters of a slot's share of a launch (with
-    // pieces of full width; the same number for every piece).
-    const int64_t total = (int64_t)(a.piece / TT) * k.rt * (nd * 2 * MP + (a.pieces > 1 ? a.dp / PK + P_TILE_EXTRA : 0));
-    const int share = (int)max((int64_t)4, total * 3 / (4 * a.slots));
-    k.xs = max(1, min((a.piece / PK + share - 1) / share, a.xcap / max(k.rt, 1)));
-    k.dw = a.dw ? nd * nv * a.wsplit : 0;
-    k.dx = a.dx && nv > 0 ? nd * k.rt * k.xs : 0;
-    // P: tiles of one token tile in strips, whose stages are one stream (MP = 2: single
-    // tiles, since their output goes through the panels).  Alone, in the rounds of equal
-    // strips that take the fewest tiles one after the other; beside the others short
-    // ones, up to four a slot.
-    const int tiles = k.rt * nvp;
-    k.strip = MP == 2 ? 1 : max(1, (tiles + P_ROUNDS * a.slots - 1) / (P_ROUNDS * a.slots));
-    if (MP == 4 && k.dw + k.dx == 0) {
-        int cost = INT32_MAX;
-        for (int r = 1; r <= P_ROUNDS; ++r) {
-            const int s = max(1, (tiles + r * a.slots - 1) / (r * a.slots));
-            const int c = (k.rt * ((nvp + s - 1) / s) + a.slots - 1) / a.slots * (4 * s + 1);   // a strip's start: a quarter tile
-            if (c < cost) {
-                cost = c;
-                k.strip = s;
-            }
-        }
-    }
-    k.p = k.rt * ((nvp + k.strip - 1) / k.strip);
-    return k;
-}
-
 // k.strip tiles of P: logits again, softmax, minus one at the target; M side
 // vocabulary rows, N side tokens.  In units of 1 / P_SCALE, times the row's factor.
 template <typename T, int MP>
@@ -661,13 +611,9 @@ hipError_t fwd(const XentArgs &a, hipStream_t st) {
 // P of [p0, p1) beside dW and dx of [v0, v1); either may be empty.
 template <typename T, int MP>
 hipError_t grad(const XentArgs &a, hipStream_t st) {
-    constexpr int TT = 64 * MP;
-    const int rt = a.rows_pad / TT, nd = (a.d + TT - 1) / TT, nv = (a.v1 - a.v0 + TT - 1) / TT, np = (a.p1 - a.p0 + TT - 1) / TT;
-    // the most items there can be
-    const int strips = MP == 2 || rt * np < P_ROUNDS * a.slots + rt ? rt * np : P_ROUNDS * a.slots + rt;
-    const int items = (a.dw ? nd * nv * a.wsplit : 0) + (a.dx && nv ? nd * a.xcap : 0) + strips;
+    const int nv = a.v1 - a.v0, items = xent_work_most<MP>(a);
     if (items > 0) FA2_LAUNCH((xent_grad_kernel<T, MP>), items, 512);
-    if (nv && a.dw && a.wsplit > 1) FA2_LAUNCH(xent_dw_join_kernel<T>, at_most((a.v1 - a.v0 + 3) / 4, 8192), 256);
+    if (nv && a.dw && a.wsplit > 1) FA2_LAUNCH(xent_dw_join_kernel<T>, at_most((nv + 3) / 4, 8192), 256);
     return hipSuccess;
 }
 
