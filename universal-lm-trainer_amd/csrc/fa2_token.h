@@ -143,7 +143,7 @@ struct XentArgs {
     int slots;                     // workgroups resident at once
     int piece, pieces;             // vocabulary columns of a piece; pieces
     int v0, v1;                    // the piece whose dW and dx are formed, from P
-    const void *P;                 // [rows_pad, piece]
+    const void *P;                 // [rows_pad / 64, piece / 64] panels of 64 x 64
     int p0, p1;                    // the piece whose P is formed, into Pn
     void *Pn;
     int xcap;                      // dx: token tiles there are sums for, in all slices

@@ -174,7 +174,7 @@ __device__ __forceinline__ void join_max_sum(float &m, float &l, float m2, float
 // of stages: the next tile's transfers run behind the exponentials.
 template <typename T, int MP, int NP, int WM, int WN, int NS>
 __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
-    typedef Product<T, true, true, false, MP == 4, MP, NP, WM, WN, NS> Pr;   // MP < 4: the states may be the caller's
+    typedef Product<T, true, true, CLAMPED, MP == 4 ? PADDED : CLAMPED, MP, NP, WM, WN, NS> Pr;   // MP < 4: the states may be the caller's
     constexpr int MI = Pr::MI, NI = Pr::NI;
     __shared__ __align__(16) char mem[Pr::LDS];
     const int n = a.direct ? (int)a.rows : a.count[N_TOKENS], splits = a.direct ? a.stat_splits : a.count[STAT_SPLITS];
@@ -366,7 +366,7 @@ __device__ __forceinline__ float xent_unscale(const XentArgs &a, int n) {
 // vocabulary rows, N side tokens.  In units of 1 / P_SCALE, times the row's factor.
 template <typename T, int MP>
 __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k, int item, int n, char *mem, char *out) {
-    typedef Product<T, true, true, false, true, MP, MP, 2, 4> Pr;
+    typedef Product<T, true, true, CLAMPED, PADDED, MP, MP, 2, 4> Pr;
     const int tiles = (a.p1 - a.p0 + Pr::TM - 1) / Pr::TM, strips = (tiles + k.strip - 1) / k.strip;
     // groups of 8 token tiles, in a group the tokens fastest
     const int g = item / (8 * strips), gs = min(8, k.rt - 8 * g), in = item - g * 8 * strips;
@@ -406,7 +406,9 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
         pr.steps(stream, a.dp / PK, acc, next);
 #pragma unroll
         for (int j = 0; j < Pr::NI; ++j) {
-            T *o = static_cast<T *>(a.Pn) + (int64_t)(rb * Pr::TN + pr.wn + 32 * j) * a.piece + t * Pr::TM + pr.wm;
+            // rows of 64 elements in panel (row / 64, (t * TM + wm) / 64 + i / 2)
+            const int row = rb * Pr::TN + pr.wn + 32 * j;
+            T *o = static_cast<T *>(a.Pn) + ((int64_t)(row >> 6) * (a.piece / 64) + ((t * Pr::TM + pr.wm) >> 6)) * 4096 + (row & 63) * 64;
 #pragma unroll
             for (int i = 0; i < Pr::MI; i += 2) {
 #pragma unroll
@@ -427,7 +429,7 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
                             if (v0 + pr.wm + 32 * (i + h) + acc_row(r, g2) >= a.V) acc[i + h][j][r] = 0.f;
                     }
                 }
-                store_rows<T>(acc[i][j], acc[i + 1][j], f[j], blk, o + 32 * i, a.piece, 32, 64, true);
+                store_rows<T>(acc[i][j], acc[i + 1][j], f[j], blk, o + (i / 2) * 4096, 64, 32, 64, true);
             }
         }
     }
@@ -437,7 +439,7 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
 // vocabulary rows, K packed tokens.
 template <typename T, int MP>
 __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n, char *mem) {
-    typedef Product<T, false, false, true, true, MP, MP, 2, 4> Pr;
+    typedef Product<T, false, false, PADDED, PANELED, MP, MP, 2, 4> Pr;
     const int nd = (a.d + Pr::TM - 1) / Pr::TM, nv = (a.v1 - a.v0 + Pr::TM - 1) / Pr::TM;
     const int db = item % nd, vb = item / nd % nv, s = item / nd / nv;
     const int kt = (n + Pr::TM - 1) / Pr::TM * MP;
@@ -445,7 +447,7 @@ __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n,
     Pr pr;
     pr.init(mem);
     pr.A.init(a.xc, a.dp, db * Pr::TM, a.dp, a.rows_pad);
-    pr.B.init(a.P, a.piece, vb * Pr::TN, a.piece, a.rows_pad);
+    pr.B.init(a.P, a.piece / 64, vb * Pr::TN);
     f16x acc[Pr::MI][Pr::NI];
     pr.run(k0, k1, acc);
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
@@ -481,14 +483,14 @@ __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n,
 // side hidden columns, K the piece.
 template <typename T, int MP>
 __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &k, int item, char *mem) {
-    typedef Product<T, true, false, true, true, MP, MP, 2, 4> Pr;
+    typedef Product<T, true, false, PANELED, PADDED, MP, MP, 2, 4> Pr;
     const int nd = (a.d + Pr::TN - 1) / Pr::TN;
     const int db = item % nd, rb = item / nd % k.rt, s = item / nd / k.rt;
     const int kt = (a.v1 - a.v0 + PK - 1) / PK;
     const int k0 = (int)((int64_t)kt * s / k.xs) * PK, k1 = (int)((int64_t)kt * (s + 1) / k.xs) * PK;
     Pr pr;
     pr.init(mem);
-    pr.A.init(a.P, a.piece, rb * Pr::TM, a.rows_pad, 0);
+    pr.A.init(a.P, a.piece / 64, rb * Pr::TM);
     pr.B.init(static_cast<const T *>(a.w) + (int64_t)a.v0 * a.w_stride, a.w_stride, db * Pr::TN, a.dp, a.V - a.v0);
     f16x acc[Pr::MI][Pr::NI];
     pr.run(k0, k1, acc);
@@ -514,7 +516,7 @@ __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &
 // an item, whose output goes through the panels.
 template <typename T, int MP>
 __global__ __launch_bounds__(512, 2) void xent_grad_kernel(const XentArgs a) {
-    constexpr int PANELS = Product<T, true, true, false, true, MP, MP, 2, 4>::LDS;
+    constexpr int PANELS = Product<T, true, true, CLAMPED, PADDED, MP, MP, 2, 4>::LDS;
     __shared__ __align__(16) char mem[PANELS + (MP == 4 ? 8 * 4096 : 0)];
     const int n = a.count[N_TOKENS];
     const XentWork k = xent_work<MP>(a, n);
