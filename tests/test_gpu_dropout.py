@@ -75,3 +75,10 @@ def test_refusals(fa):
                  lambda: fa.dropout(x[0, 0], 0.1), lambda: fa.dropout(x.cpu(), 0.1)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_probability_that_rounds_to_one_is_refused(fa):
+    x, w = torch.zeros(4, 8, device=DEV), torch.ones(8, device=DEV)
+    for call in (lambda: fa.dropout(x, 1 - 1e-9), lambda: fa.add_rms_norm(x, x, w, dropout_p=1 - 1e-9)):
+        with pytest.raises(ValueError):
+            call()

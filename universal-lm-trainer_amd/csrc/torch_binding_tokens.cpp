@@ -60,7 +60,7 @@ void check_rows(const Tensor &x, const char *op) {
 }
 
 void check_p(double p, const char *op) {
-    TORCH_CHECK_VALUE(p >= 0.0 && p < 1.0, op, ": dropout probability ", p, " outside [0, 1)");
+    TORCH_CHECK_VALUE(p >= 0.0 && (float)p < 1.f, op, ": dropout probability ", p, " outside [0, 1)");
 }
 
 // A gradient that was asked for with create_graph: an error where it is differentiated.
