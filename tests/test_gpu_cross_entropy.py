@@ -290,3 +290,18 @@ def test_forward_only(fa, n, d, V, t):
             assert not got[target == -100].any()
         total = fa.linear_cross_entropy(bad, w, target, reduction="sum")
         assert abs(total.double() - ref.double().sum()) <= 2 * e.sum()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("t", [F16, BF16])
+def test_a_gradient_that_is_not_finite_stays_in_its_row(fa, bad, t):
+    x, w, target = data(70, 128, 300, t, 12)
+    g = torch.rand(70, generator=torch.Generator().manual_seed(3)).to(DEV) + 0.5
+    g[11], g[40] = 0.0, 0.0
+    _, dx0, dw0 = run(fa, x, w, target, "none", g)
+    g[11], g[40] = bad, 0.0
+    _, dx1, dw1 = run(fa, x, w, target, "none", g)
+    others = torch.arange(70, device=DEV) != 11
+    assert torch.equal(dx1[others], dx0[others]) and not dx1[40].any()
+    assert not torch.isfinite(dx1[11]).any() and not torch.isfinite(dw1).any()
+    assert torch.isfinite(dw0).all()

@@ -39,7 +39,10 @@ constexpr int PACK_ROWS = 64;   // packed rows a workgroup has at a time, at mos
 
 // Every workgroup counts through all targets, and does its share of the rest: the
 // packed rows' token, target and states (zeros behind the last column and up to a
-// whole tile of rows), and the tokens' packed rows.
+// whole tile of rows), and the tokens' packed rows.  Counting everywhere takes no
+// second launch and no memory between workgroups: 16384 tokens x 768 in 20 us, of which
+// the copy of the states is half (50 MB); read once a workgroup, the targets come
+// from L2.
 template <typename T>
 __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
     constexpr int Q = 16;                // targets a thread has at a time
@@ -172,6 +175,13 @@ __device__ __forceinline__ void join_max_sum(float &m, float &l, float m2, float
 // the maximum of the lane's first tile and moves only when a sum passes 2^100: fp32
 // holds the terms of any larger logits until then.  The slice's tiles are one stream
 // of stages: the next tile's transfers run behind the exponentials.
+//
+// Bound by the matrix units at the board's power: 16384 tokens x 32000 x 768 in fp16
+// take 710 us, 1134 TFLOP/s, where a library product of 8192^3 reaches 1215 and both keep
+// the units busy in the same number of cycles a second.  Eight waves of 128 x 64 (four
+// of 128 x 128 with their accumulators in AGPRs: 6% slower over 8 x 1023 tokens).  Few
+// tokens: 199 x 32000 x 768 take 17 us, of which the weights' 49 MB are 10; the rest is
+// one tile's start and end, which 250 workgroups cannot hide behind another's.
 template <typename T, int MP, int NP, int WM, int WN, int NS>
 __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
     typedef Product<T, true, true, CLAMPED, MP == 4 ? PADDED : CLAMPED, MP, NP, WM, WN, NS> Pr;   // MP < 4: the states may be the caller's
@@ -334,20 +344,23 @@ __global__ __launch_bounds__(1024) void xent_sum_kernel(const XentArgs a) {
 // Backward
 // ---------------------------------------------------------------------------
 
-// none: each row of P is scaled by its gradient over the largest one, which the
-// finished products are multiplied with.  (sum and mean: every row has 1.)
+// none: each row of P is scaled by its gradient over the largest finite one, which the
+// finished products are multiplied with.  (sum and mean: every row has 1.)  A gradient
+// that is not finite makes its own row of dx not finite, and dW.
 __global__ __launch_bounds__(1024) void xent_coef_kernel(const XentArgs a) {
     __shared__ float s[16];
     const int n = a.count[N_TOKENS];
     float top = 0.f;
-    auto larger = [](float a, float b) FA2_INLINE { return (b > a || b != b) ? b : a; };
-    for (int j = threadIdx.x; j < n; j += 1024) top = larger(top, fabsf(a.g[(int64_t)a.rowmap[j] * a.g_stride]));
+    for (int j = threadIdx.x; j < n; j += 1024) {
+        const float v = fabsf(a.g[(int64_t)a.rowmap[j] * a.g_stride]);
+        top = v < INFINITY ? fmaxf(top, v) : top;
+    }
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) top = larger(top, __shfl_xor(top, o));
+    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
     __syncthreads();
     top = 0.f;
-    for (int i = 0; i < 16; ++i) top = larger(top, s[i]);
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[i]);
     for (int j = threadIdx.x; j < n; j += 1024) {
         const float v = a.g[(int64_t)a.rowmap[j] * a.g_stride];
         a.coef[j] = v == 0.f ? 0.f : v / top;
@@ -364,6 +377,8 @@ __device__ __forceinline__ float xent_unscale(const XentArgs &a, int n) {
 
 // k.strip tiles of P: logits again, softmax, minus one at the target; M side
 // vocabulary rows, N side tokens.  In units of 1 / P_SCALE, times the row's factor.
+// Formed again, since keeping 16-bit logits would take their whole matrix: one
+// product in four.  16384 tokens x 8192 columns x 768 alone: 210 us, 980 TFLOP/s.
 template <typename T, int MP>
 __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k, int item, int n, char *mem, char *out) {
     typedef Product<T, true, true, CLAMPED, PADDED, MP, MP, 2, 4> Pr;
@@ -514,6 +529,12 @@ __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &
 // MP = 4: 160 KB of LDS, one workgroup a compute unit; P's output goes through LDS of
 // its own while the next tile's stages land.  MP = 2: 64 KB, two a unit, one tile of P
 // an item, whose output goes through the panels.
+//
+// Bound by the matrix units and the board's power, and by units that idle at a launch's
+// end: 16384 tokens x 8192 columns x 768, dW and dx of a piece beside P of the next,
+// take 600 us, 1030 TFLOP/s; a last piece of 7424 columns without a P beside it 400 us,
+// 930.  Pieces of half the size: the whole gradient 17% slower; of twice the size: 3%
+// faster, for 1 GiB of scratch instead of 512 MiB.
 template <typename T, int MP>
 __global__ __launch_bounds__(512, 2) void xent_grad_kernel(const XentArgs a) {
     constexpr int PANELS = Product<T, true, true, CLAMPED, PADDED, MP, MP, 2, 4>::LDS;
