@@ -9,6 +9,8 @@
 // load of fp16, where rows are made of such; else four, loaded by a type aligned to its
 // elements only, the last piece of a row by element); a division finds its first row
 // and column, later ones are found by adding the grid's stride in rows and columns.
+// Bound by memory: 32768 x 768 in fp16 take 17 to 19 us, 5.4 to 5.8 TB/s (nontemporal
+// loads or stores change nothing).
 #include "fa2_token.h"
 
 namespace fa2 {

@@ -7,8 +7,8 @@
 //
 // Bound by memory, as the forward.  A workgroup runs over many rows and keeps its part
 // of dw in registers; the parts are summed in a second kernel in a fixed order, so that
-// results do not change from run to run.  32768 x 768, fp16 branch, fp32 residual: 72
-// us, 5.6 TB/s, and 4 us for the parts.
+// results do not change from run to run.  32768 x 768, fp16 branch, fp32 residual: 69
+// us, 5.8 TB/s, and 4 us for the parts.
 #include "fa2_token.h"
 
 namespace fa2 {

@@ -100,7 +100,8 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     const int64_t token_tiles = (rows + p.stat_tile_n - 1) / p.stat_tile_n, v_tiles = p.stat_tile_m == 256 ? v256 : v128;
     p.stat_items = (int)(token_tiles > p.stat_slots * p.stat_rounds ? token_tiles : p.stat_slots * p.stat_rounds);
     if (p.stat_items > token_tiles * v_tiles) p.stat_items = (int)(token_tiles * v_tiles);
-    // Backward.  A piece's P is at most 256 MiB (twice, with more than one piece), in equal pieces.
+    // Backward.  A piece's P is at most 256 MiB (twice, with more than one piece), or 256
+    // columns from 2^19 tokens on, in equal pieces.
     const int64_t most = clamp(((int64_t)256 << 20) / (2 * R) / XENT_PAD * XENT_PAD, XENT_PAD, 1 << 24);
     p.pieces = (int)((V + most - 1) / most);
     p.piece = (int)(((V + p.pieces - 1) / p.pieces + XENT_PAD - 1) / XENT_PAD * XENT_PAD);

@@ -205,7 +205,7 @@ class Decoder(nn.Module):
 
     def quantize(self):
         """Projections behind a norm in 8 bits from now on, in cached (serving) calls of a
-        fused model."""
+        fused model: a copy of the weights as they are, on their device."""
         if not self.fused:
             raise ValueError("8-bit projections need fused")
         for layer in self.layers:
