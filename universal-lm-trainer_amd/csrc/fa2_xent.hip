@@ -240,7 +240,8 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
                 }
                 return s;
             };
-            float s = tile_sum(ref[j] == -INFINITY ? 0.f : ref[j], sum[j], LOG2E);
+            float s = INFINITY;   // the first tile has no reference yet
+            if (t > t0) s = tile_sum(ref[j] == -INFINITY ? 0.f : ref[j], sum[j], LOG2E);
             if (__any(ref[j] == -INFINITY || !(s < 0x1p100f))) {
                 FA2_COLD_BRANCH();
                 float top = ref[j];
@@ -298,6 +299,12 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const XentArgs a) {
     float loss = 0.f;
     if (j >= 0) {
         const int t = target >= 0 && target < a.V ? (int)target : -1;
+        // The first slices' pairs are on their way while the target's row is found and read.
+        constexpr int FIRST = 4;
+        const f2 *part = reinterpret_cast<const f2 *>(a.part) + (int64_t)j * splits;
+        f2 p[FIRST];
+#pragma unroll
+        for (int q = 0; q < FIRST; ++q) p[q] = lane + 64 * q < splits ? part[lane + 64 * q] : f2{-INFINITY, 0.f};
         typedef typename vec_of<T>::v8 v8;
         const T *x = static_cast<const T *>(a.xc) + (int64_t)j * a.xc_stride;
         const T *w = static_cast<const T *>(a.w) + (int64_t)max(t, 0) * a.w_stride;
@@ -309,10 +316,9 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const XentArgs a) {
             for (int e = 0; e < 8; ++e) z += xv[e] * wv[e];
         }
         float m = -INFINITY, l = 0.f;
-        for (int s = lane; s < splits; s += 64) {
-            const f2 p = reinterpret_cast<const f2 *>(a.part)[(int64_t)j * splits + s];
-            join_max_sum(m, l, p[0], p[1]);
-        }
+#pragma unroll
+        for (int q = 0; q < FIRST; ++q) join_max_sum(m, l, p[q][0], p[q][1]);
+        for (int s = lane + 64 * FIRST; s < splits; s += 64) join_max_sum(m, l, part[s][0], part[s][1]);
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) {
             join_max_sum(m, l, __shfl_xor(m, o), __shfl_xor(l, o));
