@@ -304,7 +304,7 @@ int fa2_dropout(const fa2_dropout_params *p, void *stream);
  * or the mean over the tokens that count (NaN where there is none).
  * x, weight, dx, dweight: fp16 or bf16; dx and dweight packed; logits, log-sum-exp
  * and all sums fp32.  weight 16-byte aligned with weight_stride (below 2^22) a multiple of 8,
- * unless hidden is no multiple of 64 (then it is copied to padded rows first).
+ * unless hidden is no multiple of 8 (then it is copied to padded rows first).
  * rows <= 2^24, vocab <= 2^24, 1 <= hidden <= FA2_ROW_MAX.  Nothing is atomic:
  * results repeat bit for bit. */
 enum fa2_reduction { FA2_REDUCE_NONE = 0, FA2_REDUCE_SUM = 1, FA2_REDUCE_MEAN = 2 };

@@ -305,3 +305,24 @@ def test_a_gradient_that_is_not_finite_stays_in_its_row(fa, bad, t):
     assert torch.equal(dx1[others], dx0[others]) and not dx1[40].any()
     assert not torch.isfinite(dx1[11]).any() and not torch.isfinite(dw1).any()
     assert torch.isfinite(dw0).all()
+
+
+@pytest.mark.parametrize("n,d,V", [(1, 8, 5), (40, 72, 300), (130, 200, 4000), (300, 328, 2000), (300, 1160, 700), (700, 56, 1030),
+                                   (9000, 136, 20000)])
+@pytest.mark.parametrize("t", [F16, BF16])
+def test_rows_of_wider_matrices_whose_rest_is_nan(fa, n, d, V, t):
+    """Hidden sizes that are multiples of 8 only: tiles end inside the row, and what lies behind it is not taken."""
+    x, w, target = data(n, d, V, t, n + d)
+    wide_x = torch.full((n, d + 64), float("nan"), dtype=t, device=DEV)
+    wide_w = torch.full((V, d + 64), float("nan"), dtype=t, device=DEV)
+    wide_x[:, :d], wide_w[:, :d] = x, w
+    xs, ws = wide_x[:, :d], wide_w[:, :d]
+    with torch.no_grad():
+        assert torch.equal(fa.linear_cross_entropy(xs, ws, target, reduction="none"),
+                           fa.linear_cross_entropy(x, w, target, reduction="none"))
+    check(fa, x, w, target, g=torch.tensor(1024.0 if t == F16 else 1.0, device=DEV))
+    a = run(fa, x, w, target)
+    xs, ws = xs.detach().requires_grad_(True), ws.detach().requires_grad_(True)
+    loss = fa.linear_cross_entropy(xs, ws, target)
+    for got, want in zip((loss, *torch.autograd.grad(loss, (xs, ws))), a):
+        assert torch.equal(got, want)

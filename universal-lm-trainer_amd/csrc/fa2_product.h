@@ -59,20 +59,28 @@ struct PanelFeed {
     }
 };
 
+enum Source {
+    CLAMPED,   // the operand may end inside the tile
+    RAGGED,    // and its stored rows inside a panel
+    PADDED,    // it has every row of the tile
+    PANELED,   // it is stored in panels
+};
+
 // One operand of a tile: where the transfers of this thread read.  Eight waves
-// move a panel, wave w its rows 8 w .. 8 w + 7.  WHOLE (ROWS): the matrix has every row of
-// the tile.
-template <bool ROWS, bool WHOLE, int NP>
+// move a panel, wave w its rows 8 w .. 8 w + 7.
+template <bool ROWS, Source S, int NP>
 struct Feed {
     uint64_t base;                 // ROWS: first row, k = 0; else k = 0, column 0
     uint32_t ld;                   // bytes of a row, below 2^24
     uint32_t row, chunk;           // this lane's row of a panel; byte in the row
     int last;                      // last row there is (k row, if not ROWS), from base
+    uint32_t end;                  // RAGGED: bytes of a row
     uint32_t col[ROWS ? 1 : NP];   // not ROWS: bytes of each panel's first column
 
-    // p: the matrix; first: the tile's first row (column); limit: rows (columns, a
-    // multiple of 64) there are, at least 1 (64); k rows klimit.  What lies past a limit is
-    // read from the last row or panel there is.
+    // p: the matrix; first: the tile's first row (column); limit: rows (columns) there
+    // are; klimit: k there are.  Rows (columns) past the limit are read from the last there
+    // are, and so are k rows; k columns past theirs become zeros, whatever stands
+    // behind them.  Columns: a multiple of 8 where RAGGED, else of 64.
     __device__ __forceinline__ void init(const void *p, int64_t ld_elems, int first, int limit, int klimit) {
         const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
         row = 8 * w + (lane >> 3);
@@ -81,13 +89,16 @@ struct Feed {
             const int f0 = min(first, limit - 1);
             base = uniform64((uint64_t)(uintptr_t)p + (uint64_t)f0 * (uint64_t)ld);
             last = limit - 1 - f0;
+            end = (uint32_t)klimit * 2;
             chunk = (uint32_t)((lane & 7) ^ swz_rows(row)) << 4;
         } else {
             base = uniform64((uint64_t)(uintptr_t)p);
             last = klimit - 1;
+            end = (uint32_t)limit * 2;
             chunk = (uint32_t)((lane & 7) ^ swz_tr(row)) << 4;
 #pragma unroll
-            for (int j = 0; j < NP; ++j) col[j] = (uint32_t)min(first + 64 * j, limit - 64) * 2;
+            for (int j = 0; j < NP; ++j)
+                col[j] = (uint32_t)(S == RAGGED ? first + 64 * j : min(first + 64 * j, limit - 64)) * 2;
         }
     }
 
@@ -100,18 +111,37 @@ struct Feed {
         if constexpr (ROWS) {
             const uint64_t b = base + (uint64_t)(uint32_t)k0 * 2;
             int r = (int)row;
-            if (!WHOLE) asm volatile("" : "+v"(r));   // no offset leaves the loop
+            if (S != PADDED) asm volatile("" : "+v"(r));   // no offset leaves the loop
+            auto panels = [&]() FA2_INLINE {
 #pragma unroll
-            for (int j = 0; j < NP; ++j)
-                if (WHOLE)
-                    lds_dma16_at(b + (uint64_t)(64 * j) * ld, mul_u24(ld, (uint32_t)r) + chunk, lds + j * PANEL);
-                else
-                    lds_dma16_at(b, mul_u24(ld, (uint32_t)min(64 * j + r, last)) + chunk, lds + j * PANEL);
+                for (int j = 0; j < NP; ++j)
+                    if (S == PADDED)
+                        lds_dma16_at(b + (uint64_t)(64 * j) * ld, mul_u24(ld, (uint32_t)r) + chunk, lds + j * PANEL);
+                    else
+                        lds_dma16_at(b, mul_u24(ld, (uint32_t)min(64 * j + r, last)) + chunk, lds + j * PANEL);
+            };
+            const uint32_t left = end - (uint32_t)k0 * 2;
+            if (S != RAGGED || left >= 2 * PK) {
+                panels();
+            } else {   // every wave has lanes on both sides: it starts as many transfers as ever
+                FA2_COLD_BRANCH();
+                if (chunk < left) {
+                    panels();
+                } else {
+                    typedef __attribute__((address_space(3))) f4 lds_f4;
+#pragma unroll
+                    for (int j = 0; j < NP; ++j) *(lds_f4 *)(lds + j * PANEL + (threadIdx.x & 63) * 16) = f4{0.f, 0.f, 0.f, 0.f};
+                }
+            }
         } else {
-            const uint32_t o = mul_u24(ld, (uint32_t)min((int)row, last - k0)) + chunk;
+            const uint32_t o = mul_u24(ld, (uint32_t)min((int)row, last - k0));
             const uint64_t b = base + (uint64_t)(uint32_t)k0 * ld;
 #pragma unroll
-            for (int j = 0; j < NP; ++j) lds_dma16_at(b + col[j], o, lds + j * PANEL);
+            for (int j = 0; j < NP; ++j)
+                if (S == RAGGED)
+                    lds_dma16_at(b, o + min(col[j] + chunk, end - 16), lds + j * PANEL);
+                else
+                    lds_dma16_at(b + col[j], o + chunk, lds + j * PANEL);
         }
     }
 };
@@ -157,11 +187,6 @@ struct Frag {
 
 // Tile of 64 MP x 64 NP by eight waves in WM x WN, each (64 MP / WM) x (64 NP / WN),
 // with NS stages in LDS.
-enum Source {
-    CLAMPED,   // the operand may end inside the tile
-    PADDED,    // it has every row of the tile
-    PANELED,   // it is stored in panels
-};
 template <typename T, bool AROWS, bool BROWS, Source AS, Source BS, int MP, int NP, int WM, int WN, int NS = 2>
 struct Product {
     static_assert(WM * WN == 8, "eight waves");
@@ -170,8 +195,8 @@ struct Product {
     static constexpr int STAGE = (MP + NP) * PANEL;
     static constexpr int LDS = NS * STAGE;
 
-    typename std::conditional<AS == PANELED, PanelFeed<AROWS, MP>, Feed<AROWS, AS == PADDED, MP>>::type A;
-    typename std::conditional<BS == PANELED, PanelFeed<BROWS, NP>, Feed<BROWS, BS == PADDED, NP>>::type B;
+    typename std::conditional<AS == PANELED, PanelFeed<AROWS, MP>, Feed<AROWS, AS, MP>>::type A;
+    typename std::conditional<BS == PANELED, PanelFeed<BROWS, NP>, Feed<BROWS, BS, NP>>::type B;
     Frag<T, AROWS, TM / WM> fa;
     Frag<T, BROWS, TN / WN> fb;
     char *mem;

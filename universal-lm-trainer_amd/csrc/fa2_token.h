@@ -111,8 +111,9 @@ struct XentArgs {
     int type;
     const void *x;                 // [N, d]
     int64_t x_stride;
-    const void *w;                 // [V, dp]: the weight, or its padded copy
+    const void *w;                 // [V, wd]: the weight, wd = d, or its padded copy, wd = dp
     int64_t w_stride;
+    int wd;
     const int64_t *target;
     int64_t ignore;
     int reduction;

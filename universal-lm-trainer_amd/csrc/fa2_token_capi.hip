@@ -129,7 +129,7 @@ XentPlan xent_plan(int64_t rows, int32_t d, int32_t V) {
     p.pos = take((size_t)rows * 4);
     p.xc = take((size_t)R * p.dp * 2);
     p.state_bytes = at;
-    const size_t wbytes = d % XENT_KPAD ? (size_t)V * p.dp * 2 : 0;
+    const size_t wbytes = d % 8 ? (size_t)V * p.dp * 2 : 0;
     at = 0;
     p.f_weight = take(wbytes);
     p.part = take((size_t)p.stat_items * p.stat_tile_n * 8);
@@ -162,7 +162,7 @@ int xent_check(const fa2_xent_params *p, const void *ws, size_t ws_bytes, bool b
     if ((rc = check_row_tensor("weight", p->weight, p->type, p->weight_stride))) return rc;
     if (p->weight_stride >= 1 << 22) return fail(FA2_ERR_BAD_SHAPE, "weight row stride %lld is not below 2^22", (long long)p->weight_stride);
     if (p->weight_stride < p->hidden) return fail(FA2_ERR_BAD_SHAPE, "weight row stride %lld is below hidden", (long long)p->weight_stride);
-    if (p->hidden % fa2::XENT_KPAD == 0 && (!aligned(p->weight, 16) || p->weight_stride % 8))
+    if (p->hidden % 8 == 0 && (!aligned(p->weight, 16) || p->weight_stride % 8))
         return fail(FA2_ERR_MISALIGNED, "weight needs a 16-byte aligned base and a row stride that is a multiple of 8");
     if (p->rows > 0) {
         if (!backward && (rc = check_row_tensor("x", p->x, p->type, p->x_stride))) return rc;
@@ -193,6 +193,7 @@ fa2::XentArgs xent_args(const fa2_xent_params *p, const XentPlan &pl, char *s) {
     a.x_stride = p->x_stride;
     a.w = p->weight;
     a.w_stride = p->weight_stride;
+    a.wd = p->hidden;
     a.target = p->target;
     a.ignore = p->ignore_index;
     a.reduction = p->reduction;
@@ -350,7 +351,7 @@ int fa2_xent_fwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
     // Nothing kept, and states that the products can read: few enough tokens are not
     // packed (the weights' bytes, not the tokens, set the time), which saves a launch.
     a.direct = !p->state && p->reduction == FA2_REDUCE_NONE && pl.stat_tile_m == 128 && p->rows > 0 &&
-               p->hidden % fa2::XENT_KPAD == 0 && aligned(p->x, 16) && p->x_stride % 8 == 0 && p->x_stride < 1 << 22;
+               p->hidden % 8 == 0 && aligned(p->x, 16) && p->x_stride % 8 == 0 && p->x_stride < 1 << 22;
     if (a.direct) {
         a.xc = const_cast<void *>(p->x);
         a.xc_stride = p->x_stride;
@@ -360,10 +361,10 @@ int fa2_xent_fwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
     a.row_loss = reinterpret_cast<float *>(w + pl.row_loss);
     a.loss = p->loss;
     hipError_t e = hipSuccess;
-    if (p->hidden % fa2::XENT_KPAD) {
+    if (p->hidden % 8) {
         e = fa2::launch_xent_pad_weight(p->weight, p->weight_stride, w + pl.f_weight, a.V, a.d, a.dp, a.type, st);
         a.w = w + pl.f_weight;
-        a.w_stride = a.dp;
+        a.w_stride = a.wd = a.dp;
     }
     if (e == hipSuccess) e = fa2::launch_xent_fwd(a, st);
     return launched("cross entropy", e);
@@ -394,10 +395,10 @@ int fa2_xent_bwd(const fa2_xent_params *p, void *workspace, size_t workspace_byt
     a.dx = p->rows > 0 ? p->dx : nullptr;
     a.dw = p->dweight;
     hipError_t e = hipSuccess;
-    if (p->hidden % fa2::XENT_KPAD) {
+    if (p->hidden % 8) {
         e = fa2::launch_xent_pad_weight(p->weight, p->weight_stride, w + pl.b_weight, a.V, a.d, a.dp, a.type, st);
         a.w = w + pl.b_weight;
-        a.w_stride = a.dp;
+        a.w_stride = a.wd = a.dp;
     }
     if (e == hipSuccess && per_row) e = fa2::launch_xent_bwd_prepare(a, st);
     for (int i = 0; i <= a.pieces && e == hipSuccess; ++i) {   // P of piece i beside the gradients of piece i - 1

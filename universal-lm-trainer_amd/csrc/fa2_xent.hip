@@ -143,8 +143,8 @@ __global__ __launch_bounds__(1024) void xent_pack_kernel(const XentArgs a) {
     }
 }
 
-// Copy of the weight with rows of dp elements, for hidden sizes or strides that
-// the tiles' 16-byte loads do not take.
+// Copy of the weight with rows of dp elements, for hidden sizes that 16-byte loads do
+// not divide.
 template <typename T>
 __global__ __launch_bounds__(256) void xent_pad_weight_kernel(const T *w, int64_t stride, T *out, int V, int d, int dp) {
     for (int64_t r = blockIdx.x; r < V; r += gridDim.x)
@@ -182,9 +182,9 @@ __device__ __forceinline__ void join_max_sum(float &m, float &l, float m2, float
 // of 128 x 128 with their accumulators in AGPRs: 6% slower over 8 x 1023 tokens).  Few
 // tokens: 199 x 32000 x 768 take 17 us, of which the weights' 49 MB are 10; the rest is
 // one tile's start and end, which 250 workgroups cannot hide behind another's.
-template <typename T, int MP, int NP, int WM, int WN, int NS>
+template <typename T, Source W, int MP, int NP, int WM, int WN, int NS>
 __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
-    typedef Product<T, true, true, CLAMPED, MP == 4 ? PADDED : CLAMPED, MP, NP, WM, WN, NS> Pr;   // MP < 4: the states may be the caller's
+    typedef Product<T, true, true, W, MP == 4 ? PADDED : W, MP, NP, WM, WN, NS> Pr;   // MP < 4: the states may be the caller's
     constexpr int MI = Pr::MI, NI = Pr::NI;
     __shared__ __align__(16) char mem[Pr::LDS];
     const int n = a.direct ? (int)a.rows : a.count[N_TOKENS], splits = a.direct ? a.stat_splits : a.count[STAT_SPLITS];
@@ -198,8 +198,8 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
     Pr pr;
     pr.init(mem);
-    pr.A.init(a.w, a.w_stride, t0 * Pr::TM, a.V, 0);
-    pr.B.init(a.xc, a.xc_stride, rb * Pr::TN, a.direct ? n : a.rows_pad, 0);
+    pr.A.init(a.w, a.w_stride, t0 * Pr::TM, a.V, a.wd);
+    pr.B.init(a.xc, a.xc_stride, rb * Pr::TN, a.direct ? n : a.rows_pad, a.direct ? a.wd : a.dp);
     float ref[NI], sum[NI];
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
         nk += PK;
         if (nk == a.dp) {
             nk = 0;
-            if (++nt < t1) pr.A.init(a.w, a.w_stride, nt * Pr::TM, a.V, 0);
+            if (++nt < t1) pr.A.init(a.w, a.w_stride, nt * Pr::TM, a.V, a.wd);
         }
         return true;
     };
@@ -309,7 +309,7 @@ __global__ __launch_bounds__(256) void xent_join_kernel(const XentArgs a) {
         const T *x = static_cast<const T *>(a.xc) + (int64_t)j * a.xc_stride;
         const T *w = static_cast<const T *>(a.w) + (int64_t)max(t, 0) * a.w_stride;
         float z = 0.f;
-        for (int c = lane * 8; c < a.dp; c += 512) {
+        for (int c = lane * 8; c < a.wd; c += 512) {
             const f8 xv = __builtin_convertvector(*reinterpret_cast<const v8 *>(x + c), f8);
             const f8 wv = __builtin_convertvector(*reinterpret_cast<const v8 *>(w + c), f8);
 #pragma unroll
@@ -385,9 +385,9 @@ __device__ __forceinline__ float xent_unscale(const XentArgs &a, int n) {
 // vocabulary rows, N side tokens.  In units of 1 / P_SCALE, times the row's factor.
 // Formed again, since keeping 16-bit logits would take their whole matrix: one
 // product in four.  16384 tokens x 8192 columns x 768 alone: 210 us, 980 TFLOP/s.
-template <typename T, int MP>
+template <typename T, Source W, int MP>
 __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k, int item, int n, char *mem, char *out) {
-    typedef Product<T, true, true, CLAMPED, PADDED, MP, MP, 2, 4> Pr;
+    typedef Product<T, true, true, W, PADDED, MP, MP, 2, 4> Pr;
     const int tiles = (a.p1 - a.p0 + Pr::TM - 1) / Pr::TM, strips = (tiles + k.strip - 1) / k.strip;
     // groups of 8 token tiles, in a group the tokens fastest
     const int g = item / (8 * strips), gs = min(8, k.rt - 8 * g), in = item - g * 8 * strips;
@@ -395,8 +395,8 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
     Pr pr;
     pr.init(mem);
-    pr.A.init(a.w, a.w_stride, a.p0 + t0 * Pr::TM, a.V, 0);
-    pr.B.init(a.xc, a.dp, rb * Pr::TN, a.rows_pad, 0);
+    pr.A.init(a.w, a.w_stride, a.p0 + t0 * Pr::TM, a.V, a.wd);
+    pr.B.init(a.xc, a.dp, rb * Pr::TN, a.rows_pad, a.dp);
     float f[Pr::NI], sub[Pr::NI];
     int tgt[Pr::NI];
 #pragma unroll
@@ -414,7 +414,7 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
         nk += PK;
         if (nk == a.dp) {
             nk = 0;
-            if (++nt < t1) pr.A.init(a.w, a.w_stride, a.p0 + nt * Pr::TM, a.V, 0);
+            if (++nt < t1) pr.A.init(a.w, a.w_stride, a.p0 + nt * Pr::TM, a.V, a.wd);
         }
         return true;
     };
@@ -460,7 +460,7 @@ __device__ __forceinline__ void xent_p_item(const XentArgs &a, const XentWork &k
 // vocabulary rows, K packed tokens.
 template <typename T, int MP>
 __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n, char *mem) {
-    typedef Product<T, false, false, PADDED, PANELED, MP, MP, 2, 4> Pr;
+    typedef Product<T, false, false, CLAMPED, PANELED, MP, MP, 2, 4> Pr;
     const int nd = (a.d + Pr::TM - 1) / Pr::TM, nv = (a.v1 - a.v0 + Pr::TM - 1) / Pr::TM;
     const int db = item % nd, vb = item / nd % nv, s = item / nd / nv;
     const int kt = (n + Pr::TM - 1) / Pr::TM * MP;
@@ -502,9 +502,9 @@ __device__ __forceinline__ void xent_dw_item(const XentArgs &a, int item, int n,
 
 // A tile of the piece's share of dx, or of a slice of its k: M side packed tokens, N
 // side hidden columns, K the piece.
-template <typename T, int MP>
+template <typename T, Source W, int MP>
 __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &k, int item, char *mem) {
-    typedef Product<T, true, false, PANELED, PADDED, MP, MP, 2, 4> Pr;
+    typedef Product<T, true, false, PANELED, W, MP, MP, 2, 4> Pr;
     const int nd = (a.d + Pr::TN - 1) / Pr::TN;
     const int db = item % nd, rb = item / nd % k.rt, s = item / nd / k.rt;
     const int kt = (a.v1 - a.v0 + PK - 1) / PK;
@@ -512,7 +512,7 @@ __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &
     Pr pr;
     pr.init(mem);
     pr.A.init(a.P, a.piece / 64, rb * Pr::TM);
-    pr.B.init(static_cast<const T *>(a.w) + (int64_t)a.v0 * a.w_stride, a.w_stride, db * Pr::TN, a.dp, a.V - a.v0);
+    pr.B.init(static_cast<const T *>(a.w) + (int64_t)a.v0 * a.w_stride, a.w_stride, db * Pr::TN, a.wd, a.V - a.v0);
     f16x acc[Pr::MI][Pr::NI];
     pr.run(k0, k1, acc);
     const int lane = threadIdx.x & 63, c = lane & 31, g2 = lane >> 5;
@@ -541,9 +541,9 @@ __device__ __forceinline__ void xent_dx_item(const XentArgs &a, const XentWork &
 // take 600 us, 1030 TFLOP/s; a last piece of 7424 columns without a P beside it 400 us,
 // 930.  Pieces of half the size: the whole gradient 17% slower; of twice the size: 3%
 // faster, for 1 GiB of scratch instead of 512 MiB.
-template <typename T, int MP>
+template <typename T, Source W, int MP>
 __global__ __launch_bounds__(512, 2) void xent_grad_kernel(const XentArgs a) {
-    constexpr int PANELS = Product<T, true, true, CLAMPED, PADDED, MP, MP, 2, 4>::LDS;
+    constexpr int PANELS = Product<T, true, true, W, PADDED, MP, MP, 2, 4>::LDS;
     __shared__ __align__(16) char mem[PANELS + (MP == 4 ? 8 * 4096 : 0)];
     const int n = a.count[N_TOKENS];
     const XentWork k = xent_work<MP>(a, n);
@@ -551,11 +551,11 @@ __global__ __launch_bounds__(512, 2) void xent_grad_kernel(const XentArgs a) {
     const bool dw_first = (int64_t)n * k.xs > (int64_t)(a.v1 - a.v0) * a.wsplit;   // the longer ones
     if (dw_first && l < k.dw) return xent_dw_item<T, MP>(a, xcd_item(l, k.dw), n, mem);
     l -= dw_first ? k.dw : 0;
-    if (l < k.dx) return xent_dx_item<T, MP>(a, k, xcd_item(l, k.dx), mem);
+    if (l < k.dx) return xent_dx_item<T, W, MP>(a, k, xcd_item(l, k.dx), mem);
     l -= k.dx;
     if (!dw_first && l < k.dw) return xent_dw_item<T, MP>(a, xcd_item(l, k.dw), n, mem);
     l -= dw_first ? 0 : k.dw;
-    if (l < k.p) xent_p_item<T, MP>(a, k, xcd_item(l, k.p), n, mem, mem + (MP == 4 ? PANELS : 0));
+    if (l < k.p) xent_p_item<T, W, MP>(a, k, xcd_item(l, k.p), n, mem, mem + (MP == 4 ? PANELS : 0));
 }
 
 // Eight elements of a row of `cols`, rounded; whole 16-byte stores where `vec`.
@@ -621,29 +621,37 @@ __global__ __launch_bounds__(256) void xent_dx_out_kernel(const XentArgs a) {
         if (e != hipSuccess) return e;                                     \
     } while (0)
 
+// Hidden sizes that 64 does not divide have kernels of their own (W = RAGGED): the test
+// for a stage's end costs the others 1% of the forward.  A padded copy of the weight
+// instead: scoring of 130 tokens x 17428 x 1160 54 us, against 28.
 unsigned at_most(int64_t want, int64_t most) { return (unsigned)(want < most ? want : most); }
 
-template <typename T>
+template <typename T, Source W>
 hipError_t fwd(const XentArgs &a, hipStream_t st) {
     if (!a.direct) FA2_LAUNCH(xent_pack_kernel<T>, at_most(a.rows_pad / a.pack_rows, 1024), 1024);
     if (a.stat_tile_n == 64)
-        FA2_LAUNCH((xent_stats_kernel<T, 2, 1, 4, 2, 3>), a.stat_items, 512);
+        FA2_LAUNCH((xent_stats_kernel<T, W, 2, 1, 4, 2, 3>), a.stat_items, 512);
     else if (a.stat_tile_m == 128)
-        FA2_LAUNCH((xent_stats_kernel<T, 2, 4, 2, 4, 3>), a.stat_items, 512);
+        FA2_LAUNCH((xent_stats_kernel<T, W, 2, 4, 2, 4, 3>), a.stat_items, 512);
     else
-        FA2_LAUNCH((xent_stats_kernel<T, 4, 4, 2, 4, 2>), a.stat_items, 512);
+        FA2_LAUNCH((xent_stats_kernel<T, W, 4, 4, 2, 4, 2>), a.stat_items, 512);
     if (a.rows > 0) FA2_LAUNCH(xent_join_kernel<T>, (unsigned)((a.rows + 3) / 4), 256);
     if (a.reduction != FA2_REDUCE_NONE) FA2_LAUNCH(xent_sum_kernel, 1, 1024);
     return hipSuccess;
 }
 
 // P of [p0, p1) beside dW and dx of [v0, v1); either may be empty.
-template <typename T, int MP>
+template <typename T, Source W, int MP>
 hipError_t grad(const XentArgs &a, hipStream_t st) {
     const int nv = a.v1 - a.v0, items = xent_work_most<MP>(a);
-    if (items > 0) FA2_LAUNCH((xent_grad_kernel<T, MP>), items, 512);
+    if (items > 0) FA2_LAUNCH((xent_grad_kernel<T, W, MP>), items, 512);
     if (nv && a.dw && a.wsplit > 1) FA2_LAUNCH(xent_dw_join_kernel<T>, at_most((nv + 3) / 4, 8192), 256);
     return hipSuccess;
+}
+
+template <typename T, Source W>
+hipError_t grad_sized(const XentArgs &a, hipStream_t st) {
+    return a.small ? grad<T, W, 2>(a, st) : grad<T, W, 4>(a, st);
 }
 
 }  // namespace
@@ -660,7 +668,8 @@ hipError_t launch_xent_pad_weight(const void *w, int64_t w_stride, void *out, in
 }
 
 hipError_t launch_xent_fwd(const XentArgs &a, hipStream_t st) {
-    return a.type == FA2_F16 ? fwd<_Float16>(a, st) : fwd<__bf16>(a, st);
+    if (a.wd % PK) return a.type == FA2_F16 ? fwd<_Float16, RAGGED>(a, st) : fwd<__bf16, RAGGED>(a, st);
+    return a.type == FA2_F16 ? fwd<_Float16, CLAMPED>(a, st) : fwd<__bf16, CLAMPED>(a, st);
 }
 
 hipError_t launch_xent_bwd_prepare(const XentArgs &a, hipStream_t st) {
@@ -669,8 +678,8 @@ hipError_t launch_xent_bwd_prepare(const XentArgs &a, hipStream_t st) {
 }
 
 hipError_t launch_xent_grad(const XentArgs &a, hipStream_t st) {
-    if (a.small) return a.type == FA2_F16 ? grad<_Float16, 2>(a, st) : grad<__bf16, 2>(a, st);
-    return a.type == FA2_F16 ? grad<_Float16, 4>(a, st) : grad<__bf16, 4>(a, st);
+    if (a.wd % PK) return a.type == FA2_F16 ? grad_sized<_Float16, RAGGED>(a, st) : grad_sized<__bf16, RAGGED>(a, st);
+    return a.type == FA2_F16 ? grad_sized<_Float16, CLAMPED>(a, st) : grad_sized<__bf16, CLAMPED>(a, st);
 }
 
 hipError_t launch_xent_bwd_finish(const XentArgs &a, hipStream_t st) {

@@ -307,7 +307,7 @@ py::tuple rms_norm_fp8(const Tensor &x, const Tensor &w, double eps, const Maybe
 Tensor weight_rows(const Tensor &w) {
     const bool rows = w.stride(1) == 1 && w.stride(0) >= w.size(1) && w.stride(0) < (1 << 22);
     const bool fits = reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0 && w.stride(0) % 8 == 0;
-    if (rows && (fits || w.size(1) % 64 != 0)) return w;
+    if (rows && (fits || w.size(1) % 8 != 0)) return w;
     return w.clone(at::MemoryFormat::Contiguous);
 }
 
