@@ -180,7 +180,7 @@ __device__ __forceinline__ void join_max_sum(float &m, float &l, float m2, float
 // take 710 us, 1134 TFLOP/s, where a library product of 8192^3 reaches 1215 and both keep
 // the units busy in the same number of cycles a second.  Eight waves of 128 x 64 (four
 // of 128 x 128 with their accumulators in AGPRs: 6% slower over 8 x 1023 tokens).  Few
-// tokens: 199 x 32000 x 768 take 17 us, of which the weights' 49 MB are 10; the rest is
+// tokens: 199 x 32000 x 768 take 16.4 us, of which the weights' 49 MB are 10; the rest is
 // one tile's start and end, which 250 workgroups cannot hide behind another's.
 template <typename T, Source W, int MP, int NP, int WM, int WN, int NS>
 __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
