@@ -190,7 +190,8 @@ __global__ __launch_bounds__(512, 2) void xent_stats_kernel(const XentArgs a) {
     const int n = a.direct ? (int)a.rows : a.count[N_TOKENS], splits = a.direct ? a.stat_splits : a.count[STAT_SPLITS];
     const int rt = (n + Pr::TN - 1) / Pr::TN;
     if ((int)blockIdx.x >= rt * splits) return;
-    // groups of 8 token tiles, in a group the tokens fastest: a slice's weights meet in one XCD's L2
+    // groups of 8 token tiles, in a group the tokens fastest: a slice's weights meet in one
+    // XCD's L2 (groups of 4: equal; of 16, here and for P: the whole training call 0.6 to 1% slower)
     const int item = xcd_item(blockIdx.x, rt * splits), g = item / (8 * splits), gs = min(8, rt - 8 * g), in_g = item - g * 8 * splits;
     const int rb = 8 * g + in_g % gs, split = in_g / gs;
     const int tiles = (a.V + Pr::TM - 1) / Pr::TM;
